@@ -9,7 +9,9 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -1679,6 +1681,289 @@ int g4_attention_dev(g4_ctx *ctx, const float *d_q, const float *d_key_cache, co
   size_t o = c.add(sizeof(float) * (size_t)g4::attention_scratch_floats(a));
   G4_TRY(ensure_scratch(ctx, c.off));
   return launch_status(g4::launch_attention(a, (float *)(ctx->scratch + o), ctx->stream), "attention");
+}
+
+// ------------------------------------------------------------ paged cache ----
+
+namespace {
+
+int check_kv(const g4_kv *kv, g4::KvArgs *a) {
+  if (!kv) return fail(G4_ERR_INVALID_ARGUMENT, "cache is null");
+  if (kv->type != G4_TYPE_F32 && kv->type != G4_TYPE_F16 && kv->type != G4_TYPE_BF16)
+    return fail(G4_ERR_UNSUPPORTED, "a cache of GGML type %d (F32, F16 or BF16)", kv->type);
+  if (kv->n_layers <= 0 || kv->n_kv_heads <= 0 || kv->n_pages <= 0 || kv->max_seqs <= 0 || kv->max_pages <= 0)
+    return fail(G4_ERR_INVALID_ARGUMENT, "a cache of %d layers, %d kv heads, %d pages, %d sequences of %d pages",
+                kv->n_layers, kv->n_kv_heads, kv->n_pages, kv->max_seqs, kv->max_pages);
+  if (kv->head_size < 8 || kv->head_size > 512 || kv->head_size % 8 != 0)
+    return fail(G4_ERR_INVALID_ARGUMENT, "head size %d is not a multiple of 8 up to 512", kv->head_size);
+  const int32_t pt = kv->page_tokens;
+  if (pt < 16 || pt > 256 || (pt & (pt - 1)) != 0)
+    return fail(G4_ERR_INVALID_ARGUMENT, "pages of %d tokens (a power of two from 16 to 256)", pt);
+  if (kv->n_kv_heads > 1024 || kv->n_layers > 65536)
+    return fail(G4_ERR_INVALID_ARGUMENT, "%d kv heads or %d layers are too many", kv->n_kv_heads, kv->n_layers);
+  if (kv->max_seqs > g4::KV_MAX_SEQS)
+    return fail(G4_ERR_INVALID_ARGUMENT, "%d sequences, at most %d", kv->max_seqs, g4::KV_MAX_SEQS);
+  if ((int64_t)kv->n_pages * pt > 0x7fffffff || (int64_t)kv->max_pages * pt > (1 << 30))
+    return fail(G4_ERR_INVALID_ARGUMENT, "%d pages of %d tokens, %d a sequence: too many tokens", kv->n_pages, pt,
+                kv->max_pages);
+  if (!kv->k || !kv->v || !kv->table || !kv->lengths || !kv->refs || !kv->status)
+    return fail(G4_ERR_INVALID_ARGUMENT, "the cache holds a null pointer");
+  if (((uintptr_t)kv->k | (uintptr_t)kv->v) % 16 != 0 ||
+      ((uintptr_t)kv->table | (uintptr_t)kv->lengths | (uintptr_t)kv->refs | (uintptr_t)kv->status) % 4 != 0)
+    return fail(G4_ERR_INVALID_ARGUMENT, "the cache's k and v must be 16-byte aligned, its tables 4-byte aligned");
+  if (!a) return G4_OK;
+  a->type = kv->type;
+  a->n_layers = kv->n_layers;
+  a->n_kv = kv->n_kv_heads;
+  a->hs = kv->head_size;
+  a->page = pt;
+  a->shift = __builtin_ctz((unsigned)pt);
+  a->n_pages = kv->n_pages;
+  a->max_seqs = kv->max_seqs;
+  a->max_pages = kv->max_pages;
+  a->k = (char *)kv->k;
+  a->v = (char *)kv->v;
+  a->table = kv->table;
+  a->lengths = kv->lengths;
+  a->refs = kv->refs;
+  a->status = kv->status;
+  return G4_OK;
+}
+
+// A list of n sequences (and a second array of the same length, where there is one).
+int check_list(int32_t n, const void *d_seqs, const void *d_more) {
+  if (n < 0 || n > g4::KV_MAX_SEQS)
+    return fail(G4_ERR_INVALID_ARGUMENT, "a list of %d sequences (0 to %d)", n, g4::KV_MAX_SEQS);
+  if (n > 0 && (!d_seqs || !d_more)) return fail(G4_ERR_INVALID_ARGUMENT, "null pointer");
+  return G4_OK;
+}
+
+int check_rope(const g4_rope *r, int32_t head_size, g4::RopeArgs *a) {
+  if (r->rot < 0 || r->rot > head_size || r->rot % 2 != 0)
+    return fail(G4_ERR_INVALID_ARGUMENT, "%d rotated elements of a head of %d (an even number)", r->rot, head_size);
+  if (r->layout != G4_ROPE_HALF && r->layout != G4_ROPE_PAIRS)
+    return fail(G4_ERR_INVALID_ARGUMENT, "unknown rotary layout %d", r->layout);
+  if (r->rot > 0 && !r->freqs) return fail(G4_ERR_INVALID_ARGUMENT, "the rotary frequencies are null");
+  a->freqs = r->freqs;
+  a->rot = r->rot;
+  a->pairs = r->layout == G4_ROPE_PAIRS;
+  a->gain = r->gain;
+  return G4_OK;
+}
+
+int kv_move(g4_ctx *ctx, const g4_kv *kv, g4::KvMove m, const char *what) {
+  g4::KvArgs a;
+  G4_TRY(check_kv(kv, &a));
+  G4_TRY(check_list(m.n, m.src, m.dst));
+  if (m.n_keep < 0 || (m.n_keep > 0 && !m.keep)) return fail(G4_ERR_INVALID_ARGUMENT, "%d kept tokens", m.n_keep);
+  if ((int64_t)m.n_keep + (int64_t)m.n * kv->page_tokens > 0x7fffffff)
+    return fail(G4_ERR_INVALID_ARGUMENT, "%d kept tokens are too many", m.n_keep);
+  if (m.n == 0) return G4_OK;
+  G4_TRY(use_device(ctx));
+  Carve c;
+  const size_t o = c.add(g4::kv_move_scratch_bytes(a, m));
+  G4_TRY(ensure_scratch(ctx, c.off));
+  return launch_status(g4::launch_kv_move(a, m, ctx->scratch + o, ctx->stream), what);
+}
+
+int paged(g4_ctx *ctx, const g4_kv *kv, int32_t layer, const float *d_q, float *d_out, int32_t n_heads, int32_t n,
+          const int32_t *d_seqs, const int32_t *d_row_begin, int32_t n_rows, float scale, int32_t window,
+          int32_t sinks) {
+  g4::PagedArgs a;
+  G4_TRY(check_kv(kv, &a.kv));
+  if (layer < 0 || layer >= kv->n_layers)
+    return fail(G4_ERR_OUT_OF_RANGE, "layer %d of a cache of %d", layer, kv->n_layers);
+  if (n_heads <= 0 || n_heads > 1024 || n_heads % kv->n_kv_heads != 0)
+    return fail(G4_ERR_INVALID_ARGUMENT, "%d heads over %d kv heads (a multiple, at most 1024)", n_heads,
+                kv->n_kv_heads);
+  G4_TRY(check_list(n, d_seqs, d_seqs));
+  if (n_rows < 0 || (int64_t)n_rows * n_heads * kv->head_size > (int64_t(1) << 40))
+    return fail(G4_ERR_INVALID_ARGUMENT, "%d rows", n_rows);
+  if (window < 0 || sinks < 0) return fail(G4_ERR_INVALID_ARGUMENT, "window %d, first tokens %d", window, sinks);
+  if (!(__builtin_fabsf(scale) <= 3.4028234663852886e38f)) return fail(G4_ERR_INVALID_ARGUMENT, "the scale is not finite");
+  if (n == 0 || n_rows == 0) return G4_OK;
+  if (!d_q || !d_out) return fail(G4_ERR_INVALID_ARGUMENT, "null pointer");
+  if (((uintptr_t)d_q | (uintptr_t)d_out) % 16 != 0)
+    return fail(G4_ERR_INVALID_ARGUMENT, "q and out must be 16-byte aligned");
+  const size_t bytes = sizeof(float) * (size_t)n_rows * n_heads * kv->head_size;
+  if ((const char *)d_q < (char *)d_out + bytes && (char *)d_out < (const char *)d_q + bytes)
+    return fail(G4_ERR_INVALID_ARGUMENT, "q and out overlap");
+  G4_TRY(use_device(ctx));
+  a.layer = layer;
+  a.q = d_q;
+  a.out = d_out;
+  a.n_heads = n_heads;
+  a.n = n;
+  a.seqs = d_seqs;
+  a.row_begin = d_row_begin;
+  a.n_rows = n_rows;
+  a.scale = scale;
+  a.window = window;
+  a.sinks = sinks;
+  return launch_status(g4::launch_paged(a, ctx->dev, nullptr, ctx->stream), "paged attention");
+}
+
+}  // namespace
+
+int g4_kv_check(const g4_kv *kv) { return check_kv(kv, nullptr); }
+
+int g4_kv_init_dev(g4_ctx *ctx, const g4_kv *kv) {
+  G4_TRY(check_ctx(ctx));
+  g4::KvArgs a;
+  G4_TRY(check_kv(kv, &a));
+  G4_TRY(use_device(ctx));
+  return launch_status(g4::launch_kv_init(a, ctx->stream), "cache init");
+}
+
+int g4_kv_status(g4_ctx *ctx, const g4_kv *kv) {
+  G4_TRY(check_ctx(ctx));
+  G4_TRY(check_kv(kv, nullptr));
+  G4_TRY(use_host(ctx));
+  int32_t st = 0;
+  G4_HIP(hipMemcpyAsync(&st, kv->status, sizeof(st), hipMemcpyDeviceToHost, ctx->stream), "hipMemcpyAsync(status)");
+  G4_HIP(hipStreamSynchronize(ctx->stream), "hipStreamSynchronize");
+  if (st == g4::KV_OK) return G4_OK;
+  G4_TRY(zero_dev(ctx, kv->status, sizeof(st)));
+  G4_HIP(hipStreamSynchronize(ctx->stream), "hipStreamSynchronize");
+  if (st == g4::KV_NO_PAGES) return fail(G4_ERR_OUT_OF_MEMORY, "a call on the cache found too few free pages");
+  return fail(G4_ERR_OUT_OF_RANGE, "a call on the cache found an index, count or length out of range, or a sequence twice");
+}
+
+int g4_kv_extend_dev(g4_ctx *ctx, const g4_kv *kv, int32_t n, const int32_t *d_seqs, const int32_t *d_counts) {
+  G4_TRY(check_ctx(ctx));
+  g4::KvArgs a;
+  G4_TRY(check_kv(kv, &a));
+  G4_TRY(check_list(n, d_seqs, d_counts));
+  if (n == 0) return G4_OK;
+  G4_TRY(use_device(ctx));
+  return launch_status(g4::launch_kv_extend(a, n, d_seqs, d_counts, ctx->stream), "cache extend");
+}
+
+int g4_kv_fork_dev(g4_ctx *ctx, const g4_kv *kv, int32_t n, const int32_t *d_src, const int32_t *d_dst,
+                   const int32_t *d_lengths) {
+  G4_TRY(check_ctx(ctx));
+  return kv_move(ctx, kv, g4::KvMove{n, d_src, d_dst, d_lengths, nullptr, nullptr, 0}, "cache fork");
+}
+
+int g4_kv_compact_dev(g4_ctx *ctx, const g4_kv *kv, int32_t n, const int32_t *d_src, const int32_t *d_dst,
+                      const int32_t *d_prefix, const int32_t *d_keep, const int32_t *d_keep_begin, int32_t n_keep) {
+  G4_TRY(check_ctx(ctx));
+  if (n > 0 && !d_keep_begin) return fail(G4_ERR_INVALID_ARGUMENT, "keep_begin is null");
+  return kv_move(ctx, kv, g4::KvMove{n, d_src, d_dst, d_prefix, d_keep, d_keep_begin, n_keep}, "cache compact");
+}
+
+int g4_kv_free_dev(g4_ctx *ctx, const g4_kv *kv, int32_t n, const int32_t *d_seqs) {
+  G4_TRY(check_ctx(ctx));
+  g4::KvArgs a;
+  G4_TRY(check_kv(kv, &a));
+  G4_TRY(check_list(n, d_seqs, d_seqs));
+  if (n == 0) return G4_OK;
+  G4_TRY(use_device(ctx));
+  return launch_status(g4::launch_kv_release(a, n, d_seqs, -1, 0, ctx->stream), "cache free");
+}
+
+int g4_kv_trim_dev(g4_ctx *ctx, const g4_kv *kv, int32_t n, const int32_t *d_seqs, int32_t window, int32_t sinks) {
+  G4_TRY(check_ctx(ctx));
+  g4::KvArgs a;
+  G4_TRY(check_kv(kv, &a));
+  G4_TRY(check_list(n, d_seqs, d_seqs));
+  if (window <= 0 || sinks < 0) return fail(G4_ERR_INVALID_ARGUMENT, "window %d, first tokens %d", window, sinks);
+  if (n == 0) return G4_OK;
+  G4_TRY(use_device(ctx));
+  return launch_status(g4::launch_kv_release(a, n, d_seqs, window, sinks, ctx->stream), "cache trim");
+}
+
+int g4_rope_freqs(int32_t rot, double base, int32_t scaling, double factor, double trained, double fast, double slow,
+                  const float *divisors, double *freqs, float *gain) {
+  if (rot <= 0 || rot % 2 != 0) return fail(G4_ERR_INVALID_ARGUMENT, "%d rotated elements (an even number)", rot);
+  if (!freqs || !gain) return fail(G4_ERR_INVALID_ARGUMENT, "null pointer");
+  if (!(base > 1.0) || !std::isfinite(base)) return fail(G4_ERR_INVALID_ARGUMENT, "base %g", base);
+  if (scaling < G4_ROPE_SCALE_NONE || scaling > G4_ROPE_SCALE_RAMP)
+    return fail(G4_ERR_INVALID_ARGUMENT, "unknown scaling %d", scaling);
+  if (scaling != G4_ROPE_SCALE_NONE && !(factor >= 1.0 && std::isfinite(factor)))
+    return fail(G4_ERR_INVALID_ARGUMENT, "scaling factor %g", factor);
+  if (scaling == G4_ROPE_SCALE_BASE && rot == 2) return fail(G4_ERR_INVALID_ARGUMENT, "one pair has no base to scale");
+  if (scaling == G4_ROPE_SCALE_RAMP && !(trained > 0 && fast > slow && slow > 0 && std::isfinite(trained * fast)))
+    return fail(G4_ERR_INVALID_ARGUMENT, "trained length %g, turns %g and %g", trained, fast, slow);
+  const int n = rot / 2;
+  if (divisors)
+    for (int i = 0; i < n; ++i)
+      if (!(divisors[i] > 0.f)) return fail(G4_ERR_INVALID_ARGUMENT, "divisor %d is %g", i, divisors[i]);
+  if (scaling == G4_ROPE_SCALE_BASE) base *= std::pow(factor, rot / (rot - 2.0));
+  // pair i turns trained * base^(-2i / rot) / 2 pi times over the trained length: the
+  // (fractional) pairs that turn fast and slow times, widened to whole ones
+  double lo = 0, hi = 0;
+  if (scaling == G4_ROPE_SCALE_RAMP) {
+    auto pair_of = [&](double turns) {
+      return rot * std::log(trained / (turns * 6.283185307179586477)) / (2.0 * std::log(base));
+    };
+    lo = std::max(0.0, std::floor(pair_of(fast)));
+    hi = std::min(rot - 1.0, std::ceil(pair_of(slow)));
+  }
+  for (int i = 0; i < n; ++i) {
+    double f = std::pow(base, -2.0 * i / rot);
+    if (divisors) f /= divisors[i];
+    if (scaling == G4_ROPE_SCALE_LINEAR) f /= factor;
+    if (scaling == G4_ROPE_SCALE_RAMP) {
+      const double keep = 1.0 - std::min(1.0, std::max(0.0, (i - lo) / std::max(0.001, hi - lo)));
+      f = f * keep + f / factor * (1.0 - keep);
+    }
+    freqs[i] = f;
+  }
+  *gain = scaling == G4_ROPE_SCALE_RAMP ? (float)(1.0 + 0.1 * std::log(factor)) : 1.f;
+  return G4_OK;
+}
+
+int g4_rope_dev(g4_ctx *ctx, const g4_rope *rope, const float *d_x, float *d_out, int32_t n_rows, int32_t n_heads,
+                int32_t head_size, const int32_t *d_positions) {
+  G4_TRY(check_ctx(ctx));
+  if (!rope) return fail(G4_ERR_INVALID_ARGUMENT, "rope is null");
+  if (n_rows < 0 || n_heads <= 0 || head_size <= 0 || head_size % 2 != 0)
+    return fail(G4_ERR_INVALID_ARGUMENT, "%d rows of %d heads of %d (even)", n_rows, n_heads, head_size);
+  g4::RopeArgs r;
+  G4_TRY(check_rope(rope, head_size, &r));
+  if (n_rows == 0) return G4_OK;
+  if (!d_x || !d_out || !d_positions) return fail(G4_ERR_INVALID_ARGUMENT, "null pointer");
+  G4_TRY(use_device(ctx));
+  return launch_status(g4::launch_rope(r, d_x, d_out, n_rows, n_heads, head_size, d_positions, ctx->stream), "rope");
+}
+
+int g4_kv_rope_write_dev(g4_ctx *ctx, const g4_kv *kv, int32_t layer, const g4_rope *rope, const float *d_q,
+                         float *d_q_out, const float *d_k, const float *d_v, int32_t n_heads, int32_t n,
+                         const int32_t *d_seqs, const int32_t *d_row_begin, int32_t n_rows) {
+  G4_TRY(check_ctx(ctx));
+  g4::KvArgs a;
+  G4_TRY(check_kv(kv, &a));
+  if (layer < 0 || layer >= kv->n_layers)
+    return fail(G4_ERR_OUT_OF_RANGE, "layer %d of a cache of %d", layer, kv->n_layers);
+  if (!d_q != !d_q_out) return fail(G4_ERR_INVALID_ARGUMENT, "q without q_out");
+  if (d_q && (n_heads <= 0 || n_heads > 1024)) return fail(G4_ERR_INVALID_ARGUMENT, "%d heads", n_heads);
+  if (d_q && !rope) return fail(G4_ERR_INVALID_ARGUMENT, "queries without rotary positions");
+  G4_TRY(check_list(n, d_seqs, d_seqs));
+  if (n_rows < 0 || (!d_row_begin && n_rows != n))
+    return fail(G4_ERR_INVALID_ARGUMENT, "%d rows for %d sequences", n_rows, n);
+  g4::RopeArgs r = {nullptr, 0, 0, 1.f};
+  if (rope) G4_TRY(check_rope(rope, kv->head_size, &r));
+  if (n == 0 || n_rows == 0) return G4_OK;
+  if (!d_k || !d_v) return fail(G4_ERR_INVALID_ARGUMENT, "null pointer");
+  G4_TRY(use_device(ctx));
+  const g4::KvWrite w = {layer, d_q, d_q_out, d_k, d_v, d_q ? n_heads : 0, n, d_seqs, d_row_begin, n_rows};
+  return launch_status(g4::launch_kv_write(a, r, w, ctx->stream), "cache write");
+}
+
+int g4_paged_attention_dev(g4_ctx *ctx, const g4_kv *kv, int32_t layer, const float *d_q, float *d_out,
+                           int32_t n_heads, int32_t n, const int32_t *d_seqs, float scale, int32_t window,
+                           int32_t sinks) {
+  G4_TRY(check_ctx(ctx));
+  return paged(ctx, kv, layer, d_q, d_out, n_heads, n, d_seqs, nullptr, n, scale, window, sinks);
+}
+
+int g4_paged_prompt_dev(g4_ctx *ctx, const g4_kv *kv, int32_t layer, const float *d_q, float *d_out, int32_t n_heads,
+                        int32_t n, const int32_t *d_seqs, const int32_t *d_row_begin, int32_t n_rows, float scale,
+                        int32_t window, int32_t sinks) {
+  G4_TRY(check_ctx(ctx));
+  if (n > 0 && !d_row_begin) return fail(G4_ERR_INVALID_ARGUMENT, "row_begin is null");
+  return paged(ctx, kv, layer, d_q, d_out, n_heads, n, d_seqs, d_row_begin, n_rows, scale, window, sinks);
 }
 
 }  // extern "C"

@@ -220,4 +220,85 @@ void attention_plan(AttArgs &a, const DevInfo &dev);
 int64_t attention_scratch_floats(const AttArgs &a);
 hipError_t launch_attention(AttArgs a, float *scratch, hipStream_t stream);
 
+// A paged key-value cache (g4_kv of g4hip.h).  Device data that a call finds out of
+// range (pages, sequences, lengths) is never followed: kernels bound every index.
+struct KvArgs {
+  int32_t type;
+  int32_t n_layers;
+  int32_t n_kv;
+  int32_t hs;
+  int32_t page;   // tokens of a page, 1 << shift
+  int32_t shift;
+  int32_t n_pages;
+  int32_t max_seqs;
+  int32_t max_pages;
+  char *k;
+  char *v;
+  int32_t *table;
+  int32_t *lengths;
+  int32_t *refs;
+  int32_t *status;
+};
+// What *status holds after a call that could not be done.
+enum : int { KV_OK = 0, KV_NO_PAGES = 1, KV_BAD_DATA = 2 };
+constexpr int KV_MAX_SEQS = 1024;  // of a cache, and so of a call's list: one per thread of a workgroup
+
+hipError_t launch_kv_init(const KvArgs &kv, hipStream_t s);
+hipError_t launch_kv_extend(const KvArgs &kv, int32_t n, const int32_t *seqs, const int32_t *counts, hipStream_t s);
+// window < 0: all pages and the length; otherwise the pages that no later position sees.
+hipError_t launch_kv_release(const KvArgs &kv, int32_t n, const int32_t *seqs, int32_t window, int32_t sinks,
+                             hipStream_t s);
+struct KvMove {
+  int32_t n;
+  const int32_t *src;
+  const int32_t *dst;
+  const int32_t *prefix;  // null: the whole sequence, with listed tokens none of it
+  const int32_t *keep;
+  const int32_t *keep_begin;  // null: no listed tokens
+  int32_t n_keep;
+};
+size_t kv_move_scratch_bytes(const KvArgs &kv, const KvMove &m);
+hipError_t launch_kv_move(const KvArgs &kv, const KvMove &m, char *scratch, hipStream_t s);
+
+// Rotary positions: pair i of the first `rot` elements turned by position * freqs[i].
+struct RopeArgs {
+  const double *freqs;
+  int32_t rot;
+  int32_t pairs;  // 1: elements (2i, 2i + 1); 0: (i, i + rot / 2)
+  float gain;
+};
+hipError_t launch_rope(const RopeArgs &r, const float *x, float *out, int32_t n_rows, int32_t n_heads, int32_t hs,
+                       const int32_t *positions, hipStream_t s);
+// q (may be null) rotated to q_out; k rotated and v written as rows of the cache.
+struct KvWrite {
+  int32_t layer;
+  const float *q;
+  float *q_out;
+  const float *k;
+  const float *v;
+  int32_t n_heads;
+  int32_t n;
+  const int32_t *seqs;
+  const int32_t *row_begin;  // null: one row per sequence
+  int32_t n_rows;
+};
+hipError_t launch_kv_write(const KvArgs &kv, const RopeArgs &r, const KvWrite &w, hipStream_t s);
+
+// Attention over a layer of a paged cache.
+struct PagedArgs {
+  KvArgs kv;
+  int32_t layer;
+  const float *q;
+  float *out;
+  int32_t n_heads;
+  int32_t n;
+  const int32_t *seqs;
+  const int32_t *row_begin;  // null: one row per sequence
+  int32_t n_rows;
+  float scale;
+  int32_t window;  // 0: none
+  int32_t sinks;
+};
+hipError_t launch_paged(const PagedArgs &a, const DevInfo &dev, char *scratch, hipStream_t s);
+
 }  // namespace g4

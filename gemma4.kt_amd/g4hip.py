@@ -122,6 +122,20 @@ SIGNATURES = {
     "g4_lm_head": [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, ctypes.c_float, ctypes.c_float],
     "g4_lm_head_dev": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, ctypes.c_float, ctypes.c_float],
     "g4_attention_dev": [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32],
+    "g4_kv_check": [_vp],
+    "g4_kv_init_dev": [_vp, _vp],
+    "g4_kv_status": [_vp, _vp],
+    "g4_kv_extend_dev": [_vp, _vp, _i32, _vp, _vp],
+    "g4_kv_fork_dev": [_vp, _vp, _i32, _vp, _vp, _vp],
+    "g4_kv_compact_dev": [_vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32],
+    "g4_kv_free_dev": [_vp, _vp, _i32, _vp],
+    "g4_kv_trim_dev": [_vp, _vp, _i32, _vp, _i32, _i32],
+    "g4_rope_freqs": [_i32, ctypes.c_double, _i32, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double,
+                      _vp, _vp, _vp],
+    "g4_rope_dev": [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp],
+    "g4_kv_rope_write_dev": [_vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _i32],
+    "g4_paged_attention_dev": [_vp, _vp, _i32, _vp, _vp, _i32, _i32, _vp, ctypes.c_float, _i32, _i32],
+    "g4_paged_prompt_dev": [_vp, _vp, _i32, _vp, _vp, _i32, _i32, _vp, _vp, _i32, ctypes.c_float, _i32, _i32],
 }
 
 
@@ -646,3 +660,227 @@ def attention_dev(ctx: Context, q, key_cache, value_cache, out, n_heads: int, n_
     check(lib().g4_attention_dev(ctx.handle, _ptr(_dev_f32(q, "q")), _ptr(_dev_f32(key_cache, "key_cache")),
                                  _ptr(_dev_f32(value_cache, "value_cache")), _ptr(_dev_f32(out, "out")),
                                  int(n_heads), int(n_kv_heads), int(head_size), int(position), int(att_start)))
+
+
+# ------------------------------------------------------------ paged cache ---
+# Keys and values of several sequences in shared pages, with rotary positions and
+# attention over them (include/g4hip.h states the layout and each call's semantics).
+
+ROPE_HALF = 0    # pair i is elements i and i + rot / 2
+ROPE_PAIRS = 1   # pair i is elements 2i and 2i + 1
+
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_BASE, ROPE_SCALE_RAMP = range(4)
+
+
+def _dev(ctx: Context, t, dtype: str, n: int, name: str) -> int:
+    """Address of a contiguous tensor of torch's `dtype` on the context's device that
+    holds at least n elements (a raw device address as int passes unchecked)."""
+    if type(t) is int:
+        return t
+    import torch
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is getattr(torch, dtype) and t.is_contiguous()):
+        raise IllegalArgumentException("%s must be a contiguous %s device tensor" % (name, dtype))
+    if t.get_device() != ctx.ordinal:
+        raise IllegalArgumentException("%s lives on device %d, the context on %d" % (name, t.get_device(), ctx.ordinal))
+    if t.numel() < n:
+        raise IndexOutOfBoundsException("%s holds %d elements, %d needed" % (name, t.numel(), n))
+    return t.data_ptr()
+
+
+def _dev_list(ctx: Context, t, name: str):
+    """A list of sequences: its address and its length."""
+    if type(t) is int:
+        raise IllegalArgumentException("%s must be a device tensor, whose length is the list's" % name)
+    return _dev(ctx, t, "int32", 0, name), t.numel()
+
+
+class _KvStruct(ctypes.Structure):
+    _fields_ = ([(f, _i32) for f in ("type", "n_layers", "n_kv_heads", "head_size", "page_tokens", "n_pages",
+                                     "max_seqs", "max_pages")]
+                + [(f, _vp) for f in ("k", "v", "table", "lengths", "refs", "status")])
+
+
+class _RopeStruct(ctypes.Structure):
+    _fields_ = [("freqs", _vp), ("rot", _i32), ("layout", _i32), ("gain", ctypes.c_float)]
+
+
+class KvCache:
+    """A paged cache over the caller's device tensors: k, v [layers, pages, kv heads,
+    tokens of a page, head size] (float32, float16 or bfloat16), table [sequences,
+    pages of a sequence], lengths [sequences], refs [pages] and status [1], all int32."""
+
+    def __init__(self, k, v, table, lengths, refs, status):
+        import torch
+        types = {torch.float32: GGMLType.F32, torch.float16: GGMLType.F16, torch.bfloat16: GGMLType.BF16}
+        for name, t in (("k", k), ("v", v), ("table", table), ("lengths", lengths), ("refs", refs),
+                        ("status", status)):
+            if not (isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous()):
+                raise IllegalArgumentException("%s must be a contiguous device tensor" % name)
+            if t.device != k.device:
+                raise IllegalArgumentException("%s lives on %s, k on %s" % (name, t.device, k.device))
+        if k.dtype not in types:
+            raise UnsupportedOperationException("a cache of %s" % k.dtype)
+        if k.dim() != 5 or v.shape != k.shape or v.dtype != k.dtype:
+            raise IllegalArgumentException("k and v must be alike: [layers, pages, kv heads, tokens, head size]")
+        if any(t.dtype != torch.int32 for t in (table, lengths, refs, status)):
+            raise IllegalArgumentException("table, lengths, refs and status must be int32")
+        if table.dim() != 2 or lengths.numel() != table.shape[0] or refs.numel() != k.shape[1] or status.numel() < 1:
+            raise IllegalArgumentException("table [sequences, pages], lengths [sequences], refs [pages], status [1]")
+        self.tensors = (k, v, table, lengths, refs, status)  # kept alive with the cache
+        self.k, self.v, self.table, self.lengths, self.refs, self.status_word = self.tensors
+        self.ordinal = k.get_device()
+        self.n_layers, self.n_pages, self.n_kv_heads, self.page_tokens, self.head_size = k.shape
+        s = _KvStruct(int(types[k.dtype]), self.n_layers, self.n_kv_heads, self.head_size, self.page_tokens,
+                      self.n_pages, table.shape[0], table.shape[1], *(t.data_ptr() for t in self.tensors))
+        self._struct, self._ref = s, ctypes.addressof(s)
+        check(lib().g4_kv_check(self._ref))
+
+    @staticmethod
+    def create(ctx: Context, n_layers: int, n_kv_heads: int, head_size: int, page_tokens: int, n_pages: int,
+               max_seqs: int, max_pages: int, dtype=None) -> "KvCache":
+        """An empty cache in new tensors (dtype: a torch type, bfloat16 by default)."""
+        import torch
+        dev = torch.device("cuda", ctx.ordinal)
+        shape = (n_layers, n_pages, n_kv_heads, page_tokens, head_size)
+        k, v = (torch.zeros(shape, dtype=dtype or torch.bfloat16, device=dev) for _ in range(2))
+        i32 = dict(dtype=torch.int32, device=dev)
+        return KvCache(k, v, torch.full((max_seqs, max_pages), -1, **i32), torch.zeros(max_seqs, **i32),
+                       torch.zeros(n_pages, **i32), torch.zeros(1, **i32))
+
+    def on(self, ctx: Context) -> int:
+        """Address of the description, for a call of `ctx`."""
+        if ctx.ordinal != self.ordinal:
+            raise IllegalArgumentException("the cache lives on device %d, the context on %d" % (self.ordinal, ctx.ordinal))
+        return self._ref
+
+
+class Rope:
+    """Rotary positions: freqs is a float64 device tensor, one angle per position for
+    each pair; layout ROPE_HALF or ROPE_PAIRS; cosines and sines are multiplied by gain."""
+
+    def __init__(self, freqs, layout: int = ROPE_HALF, gain: float = 1.0):
+        import torch
+        if not (isinstance(freqs, torch.Tensor) and freqs.is_cuda and freqs.dtype == torch.float64
+                and freqs.is_contiguous() and freqs.dim() == 1):
+            raise IllegalArgumentException("freqs must be a contiguous float64 device tensor")
+        self.freqs, self.ordinal = freqs, freqs.get_device()
+        self._struct = _RopeStruct(freqs.data_ptr(), 2 * freqs.numel(), int(layout), float(gain))
+        self._ref = ctypes.addressof(self._struct)
+
+    @staticmethod
+    def create(ctx: Context, rot: int, base: float = 10000.0, layout: int = ROPE_HALF, scaling: int = ROPE_SCALE_NONE,
+               factor: float = 1.0, trained: float = 0.0, fast: float = 32.0, slow: float = 1.0,
+               divisors: Optional[np.ndarray] = None) -> "Rope":
+        """Frequencies base^(-2i / rot) under a scaling (rope_freqs), in device memory."""
+        import torch
+        freqs, gain = rope_freqs(rot, base, scaling, factor, trained, fast, slow, divisors)
+        return Rope(torch.from_numpy(freqs).to(torch.device("cuda", ctx.ordinal)), layout, gain)
+
+    def on(self, ctx: Context) -> int:
+        if ctx.ordinal != self.ordinal:
+            raise IllegalArgumentException("freqs live on device %d, the context on %d" % (self.ordinal, ctx.ordinal))
+        return self._ref
+
+
+def rope_freqs(rot: int, base: float = 10000.0, scaling: int = ROPE_SCALE_NONE, factor: float = 1.0,
+               trained: float = 0.0, fast: float = 32.0, slow: float = 1.0, divisors: Optional[np.ndarray] = None):
+    """(frequencies [rot / 2] in float64, gain) of the header's g4_rope_freqs."""
+    freqs = np.zeros(max(0, int(rot)) // 2, dtype=np.float64)
+    gain = np.zeros(1, dtype=np.float32)
+    if divisors is not None:
+        _f32(divisors, "divisors")
+        _need(divisors, freqs.size, "divisors")
+    check(lib().g4_rope_freqs(int(rot), float(base), int(scaling), float(factor), float(trained), float(fast),
+                              float(slow), _ptr(divisors), _ptr(freqs), _ptr(gain)))
+    return freqs, float(gain[0])
+
+
+def kv_init_dev(ctx: Context, cache: KvCache) -> None:
+    """Empty the cache: every page free, no sequence."""
+    check(lib().g4_kv_init_dev(ctx.handle, cache.on(ctx)))
+
+
+def kv_status(ctx: Context, cache: KvCache) -> None:
+    """Wait for the context's stream; raise what a call on the cache could not do
+    (OutOfMemoryError: too few free pages, IndexOutOfBoundsException: bad indices)."""
+    check(lib().g4_kv_status(ctx.handle, cache.on(ctx)))
+
+
+def kv_extend_dev(ctx: Context, cache: KvCache, seqs, counts) -> None:
+    """Sequence seqs[i] grows by counts[i] tokens."""
+    at, n = _dev_list(ctx, seqs, "seqs")
+    check(lib().g4_kv_extend_dev(ctx.handle, cache.on(ctx), n, at, _dev(ctx, counts, "int32", n, "counts")))
+
+
+def kv_fork_dev(ctx: Context, cache: KvCache, src, dst, lengths=None) -> None:
+    """Sequence dst[i] becomes the first lengths[i] tokens (None: all) of src[i]."""
+    at, n = _dev_list(ctx, src, "src")
+    check(lib().g4_kv_fork_dev(ctx.handle, cache.on(ctx), n, at, _dev(ctx, dst, "int32", n, "dst"),
+                               None if lengths is None else _dev(ctx, lengths, "int32", n, "lengths")))
+
+
+def kv_compact_dev(ctx: Context, cache: KvCache, src, dst, prefix, keep, keep_begin) -> None:
+    """Sequence dst[i] becomes the first prefix[i] tokens (prefix None: none) of src[i]
+    and then its tokens keep[keep_begin[i] : keep_begin[i + 1]]."""
+    at, n = _dev_list(ctx, src, "src")
+    keep_at, n_keep = _dev_list(ctx, keep, "keep")
+    check(lib().g4_kv_compact_dev(ctx.handle, cache.on(ctx), n, at, _dev(ctx, dst, "int32", n, "dst"),
+                                  None if prefix is None else _dev(ctx, prefix, "int32", n, "prefix"), keep_at,
+                                  _dev(ctx, keep_begin, "int32", n + 1, "keep_begin"), n_keep))
+
+
+def kv_free_dev(ctx: Context, cache: KvCache, seqs) -> None:
+    """Give the sequences' pages back."""
+    at, n = _dev_list(ctx, seqs, "seqs")
+    check(lib().g4_kv_free_dev(ctx.handle, cache.on(ctx), n, at))
+
+
+def kv_trim_dev(ctx: Context, cache: KvCache, seqs, window: int, sinks: int = 0) -> None:
+    """Give back the pages that no later token sees under the window and first tokens."""
+    at, n = _dev_list(ctx, seqs, "seqs")
+    check(lib().g4_kv_trim_dev(ctx.handle, cache.on(ctx), n, at, int(window), int(sinks)))
+
+
+def rope_dev(ctx: Context, rope: Rope, x, out, n_rows: int, n_heads: int, head_size: int, positions) -> None:
+    """out[r] = the heads of x[r] turned to positions[r] (out may be x)."""
+    size = n_rows * n_heads * head_size
+    check(lib().g4_rope_dev(ctx.handle, rope.on(ctx), _dev(ctx, x, "float32", size, "x"),
+                            _dev(ctx, out, "float32", size, "out"), int(n_rows), int(n_heads), int(head_size),
+                            _dev(ctx, positions, "int32", n_rows, "positions")))
+
+
+def kv_rope_write_dev(ctx: Context, cache: KvCache, layer: int, q, q_out, k, v, n_heads: int, rope: Optional[Rope],
+                      seqs, row_begin, n_rows: int) -> None:
+    """Turn q to q_out (both None: no queries) and k, and write k and v as the last rows
+    of their sequences in a layer (row_begin None: one row per sequence)."""
+    at, n = _dev_list(ctx, seqs, "seqs")
+    size = n_rows * n_heads * cache.head_size
+    kv_size = n_rows * cache.n_kv_heads * cache.head_size
+    check(lib().g4_kv_rope_write_dev(
+        ctx.handle, cache.on(ctx), int(layer), None if rope is None else rope.on(ctx),
+        None if q is None else _dev(ctx, q, "float32", size, "q"),
+        None if q_out is None else _dev(ctx, q_out, "float32", size, "q_out"),
+        _dev(ctx, k, "float32", kv_size, "k"), _dev(ctx, v, "float32", kv_size, "v"), int(n_heads), n, at,
+        None if row_begin is None else _dev(ctx, row_begin, "int32", n + 1, "row_begin"), int(n_rows)))
+
+
+def paged_attention_dev(ctx: Context, cache: KvCache, layer: int, q, out, n_heads: int, seqs, scale: float = 1.0,
+                        window: int = 0, sinks: int = 0) -> None:
+    """Attention of the last token of each sequence, q and out [n, n_heads, head size];
+    with a window, of the last `window` tokens and the first `sinks`."""
+    at, n = _dev_list(ctx, seqs, "seqs")
+    size = n * n_heads * cache.head_size
+    check(lib().g4_paged_attention_dev(ctx.handle, cache.on(ctx), int(layer), _dev(ctx, q, "float32", size, "q"),
+                                       _dev(ctx, out, "float32", size, "out"), int(n_heads), n, at, float(scale),
+                                       int(window), int(sinks)))
+
+
+def paged_prompt_dev(ctx: Context, cache: KvCache, layer: int, q, out, n_heads: int, seqs, row_begin, n_rows: int,
+                     scale: float = 1.0, window: int = 0, sinks: int = 0) -> None:
+    """The same for the last row_begin[i + 1] - row_begin[i] tokens of sequence seqs[i]."""
+    at, n = _dev_list(ctx, seqs, "seqs")
+    size = n_rows * n_heads * cache.head_size
+    check(lib().g4_paged_prompt_dev(ctx.handle, cache.on(ctx), int(layer), _dev(ctx, q, "float32", size, "q"),
+                                    _dev(ctx, out, "float32", size, "out"), int(n_heads), n, at,
+                                    _dev(ctx, row_begin, "int32", n + 1, "row_begin"), int(n_rows), float(scale),
+                                    int(window), int(sinks)))

@@ -279,6 +279,147 @@ int g4_attention_dev(g4_ctx *ctx, const float *d_q, const float *d_key_cache, co
                      float *d_out, int32_t n_heads, int32_t n_kv_heads, int32_t head_size, int32_t position,
                      int32_t att_start);
 
+/* ---- Paged key-value cache of several sequences, and the operators on it. ----
+ * The reference keeps one sequence's keys and values in contiguous fp32 rows
+ * (Llama.kt:190-218); a program that serves several shares pages between them.
+ * The caller owns the memory (all of it device memory of the context's device):
+ *   k, v     [n_layers][n_pages][n_kv_heads][page_tokens][head_size] of `type`
+ *            (F32, F16 or BF16), 16-byte aligned
+ *   table    int32 [max_seqs][max_pages]: the page of tokens j * page_tokens .. of
+ *            a sequence, -1 where there is none
+ *   lengths  int32 [max_seqs]: tokens of each sequence (0: none)
+ *   refs     int32 [n_pages]: sequences that hold a page (0: free)
+ *   status   int32 [1]
+ * head_size is a multiple of 8 up to 512, page_tokens a power of two from 16 to 256,
+ * max_seqs at most 1024, n_pages * page_tokens below 2^31 and max_pages *
+ * page_tokens at most 2^30.  Full pages may be shared; a partly filled one has one
+ * owner (the calls below keep it so).
+ *
+ * The calls take lists of sequences, and lengths change, in device memory: a
+ * captured step advances when it is replayed.  A list names no more than 1024
+ * sequences.  What a call finds there cannot be returned by it: a call that cannot
+ * be done leaves the cache as it was and sets *status (1: not enough free pages, 2: an
+ * index, count or length out of range, or a sequence twice), and while that is set
+ * every call on the cache, attention too, does nothing.  g4_kv_status reads and
+ * clears it.  Pages and lengths out of range are never followed: attention takes
+ * such a page's tokens as not there.
+ * Calls on one cache from several streams are the caller's to order. */
+typedef struct g4_kv {
+  int32_t type;
+  int32_t n_layers;
+  int32_t n_kv_heads;
+  int32_t head_size;
+  int32_t page_tokens;
+  int32_t n_pages;
+  int32_t max_seqs;
+  int32_t max_pages;
+  void *k;
+  void *v;
+  int32_t *table;
+  int32_t *lengths;
+  int32_t *refs;
+  int32_t *status;
+} g4_kv;
+
+/* Host-only validation of a cache's description: the status the calls would return
+ * (G4_ERR_UNSUPPORTED for another type).  Needs no device. */
+int g4_kv_check(const g4_kv *kv);
+/* An empty cache: every page free, no sequence. */
+int g4_kv_init_dev(g4_ctx *ctx, const g4_kv *kv);
+/* Waits for the context's stream and returns what *status held, which is cleared: G4_OK,
+ * G4_ERR_OUT_OF_MEMORY (1) or G4_ERR_OUT_OF_RANGE (2).  Not under capture. */
+int g4_kv_status(g4_ctx *ctx, const g4_kv *kv);
+/* Sequence d_seqs[i] grows by d_counts[i] >= 0 tokens, whose rows are then to be
+ * written (g4_kv_rope_write_dev, layer by layer).  Fresh pages are the lowest free
+ * ones, in the order of the list.  One launch. */
+int g4_kv_extend_dev(g4_ctx *ctx, const g4_kv *kv, int32_t n, const int32_t *d_seqs, const int32_t *d_counts);
+/* Sequence d_dst[i] becomes the first d_lengths[i] tokens of d_src[i] (d_lengths NULL:
+ * all of them): whole pages are shared, a partly used last page is copied to a fresh
+ * one, in all layers, and what d_dst[i] held is given back.  A sequence may be the
+ * source of several and itself be replaced (beams that are reordered): all read the
+ * state before the call.  d_src[i] = d_dst[i] shortens, and copies nothing where the last
+ * page is its own.  Fresh pages are free before the call.  Two launches. */
+int g4_kv_fork_dev(g4_ctx *ctx, const g4_kv *kv, int32_t n, const int32_t *d_src, const int32_t *d_dst,
+                   const int32_t *d_lengths);
+/* Sequence d_dst[i] becomes the first d_prefix[i] tokens of d_src[i] (d_prefix NULL: none),
+ * shared and copied as by g4_kv_fork_dev, followed by its tokens d_keep[j] for j in
+ * [d_keep_begin[i], d_keep_begin[i + 1]), copied to fresh pages.  d_keep_begin has n + 1
+ * rising entries from 0 to at most n_keep.  Keys keep the positions they were rotated
+ * to.  Three launches. */
+int g4_kv_compact_dev(g4_ctx *ctx, const g4_kv *kv, int32_t n, const int32_t *d_src, const int32_t *d_dst,
+                      const int32_t *d_prefix, const int32_t *d_keep, const int32_t *d_keep_begin, int32_t n_keep);
+/* The sequences' pages are given back; their length is 0. */
+int g4_kv_free_dev(g4_ctx *ctx, const g4_kv *kv, int32_t n, const int32_t *d_seqs);
+/* The pages are given back that no later token sees under a window and `sinks` first
+ * tokens (see g4_paged_attention_dev).  Lengths stay.  For sequences whose last rows
+ * have been attended to, before they are extended. */
+int g4_kv_trim_dev(g4_ctx *ctx, const g4_kv *kv, int32_t n, const int32_t *d_seqs, int32_t window, int32_t sinks);
+
+/* Rotary positions.  Pair i < rot / 2 of a head's first `rot` elements is turned by
+ * the angle position * freqs[i], and multiplied by gain; the other elements stay.
+ * G4_ROPE_HALF: pair i is elements i and i + rot / 2; G4_ROPE_PAIRS: 2i and 2i + 1.
+ * Angles are formed in double precision.  (RotaryPositionEmbeddings.kt:7-54 are the
+ * reference's tables.) */
+#define G4_ROPE_HALF 0
+#define G4_ROPE_PAIRS 1
+typedef struct g4_rope {
+  const double *freqs; /* device memory, rot / 2 entries */
+  int32_t rot;         /* even, at most head_size */
+  int32_t layout;
+  float gain;
+} g4_rope;
+
+/* How positions beyond the trained length are scaled, by `factor` >= 1:
+ * NONE    freqs[i] = base^(-2i / rot)
+ * LINEAR  those / factor
+ * BASE    with base * factor^(rot / (rot - 2)) (rot > 2)
+ * RAMP    pairs that turn more than `fast` times over the `trained` length keep their
+ *         frequency, those that turn less than `slow` times are divided by factor, with
+ *         a linear ramp over i between; gain = 1 + ln(factor) / 10 */
+#define G4_ROPE_SCALE_NONE 0
+#define G4_ROPE_SCALE_LINEAR 1
+#define G4_ROPE_SCALE_BASE 2
+#define G4_ROPE_SCALE_RAMP 3
+/* Host only: the frequencies and gain of g4_rope.  divisors (NULL, or rot / 2 positive
+ * floats) divide the unscaled frequencies. */
+int g4_rope_freqs(int32_t rot, double base, int32_t scaling, double factor, double trained, double fast, double slow,
+                  const float *divisors, double *freqs, float *gain);
+/* d_out[r] = the heads of d_x[r] turned to d_positions[r]: [n_rows][n_heads][head_size],
+ * head_size even.  d_out may be d_x.  One launch. */
+int g4_rope_dev(g4_ctx *ctx, const g4_rope *rope, const float *d_x, float *d_out, int32_t n_rows, int32_t n_heads,
+                int32_t head_size, const int32_t *d_positions);
+/* The new rows of a layer: sequence d_seqs[i] owns rows d_row_begin[i] ..
+ * d_row_begin[i + 1] - 1 of n_rows (d_row_begin, n + 1 rising entries; NULL: row i), which
+ * are its last tokens, so that row j stands at position length - rows + j.
+ * d_q [n_rows][n_heads][head_size] is turned to d_q_out (which may be d_q; both NULL: no
+ * queries), d_k [n_rows][n_kv_heads][head_size] is turned and d_v taken as it is, and
+ * both are written to the sequence's pages, rounded to nearest (F16 overflows to
+ * infinity).  rope NULL: nothing is turned, and d_q is NULL.  Rows of no sequence
+ * are left as they are.  A row whose page is not there or is shared is not written,
+ * and *status is set.  A sequence is named once.  One launch. */
+int g4_kv_rope_write_dev(g4_ctx *ctx, const g4_kv *kv, int32_t layer, const g4_rope *rope, const float *d_q,
+                         float *d_q_out, const float *d_k, const float *d_v, int32_t n_heads, int32_t n,
+                         const int32_t *d_seqs, const int32_t *d_row_begin, int32_t n_rows);
+
+/* Decode attention over the cache (Llama.kt:198-218 for every sequence of a list): row
+ * i of d_q and d_out [n][n_heads][head_size] is the last token of sequence d_seqs[i], at
+ * position p = length - 1.  Head h reads kv head h / (n_heads / n_kv_heads).  With
+ * scores s_t = scale * q . K[t],
+ *   out = sum_t exp(s_t - max) V[t] / sum_t exp(s_t - max)
+ * over the tokens t <= p that it sees: all (window = 0), or t > p - window and the
+ * first `sinks`.  A row that sees nothing (an empty sequence, pages given back, scores
+ * that are all -infinity) is zeros.  fp32 products and sums.  d_q and d_out are 16-byte
+ * aligned and do not overlap. */
+int g4_paged_attention_dev(g4_ctx *ctx, const g4_kv *kv, int32_t layer, const float *d_q, float *d_out,
+                           int32_t n_heads, int32_t n, const int32_t *d_seqs, float scale, int32_t window,
+                           int32_t sinks);
+/* The same for several tokens per sequence (prompts, their chunks, drafted tokens): the
+ * rows of each sequence as in g4_kv_rope_write_dev, each at its own position and seeing
+ * no later one.  Rows of no sequence are left as they are. */
+int g4_paged_prompt_dev(g4_ctx *ctx, const g4_kv *kv, int32_t layer, const float *d_q, float *d_out, int32_t n_heads,
+                        int32_t n, const int32_t *d_seqs, const int32_t *d_row_begin, int32_t n_rows, float scale,
+                        int32_t window, int32_t sinks);
+
 #ifdef __cplusplus
 }
 #endif
