@@ -1800,7 +1800,10 @@ int paged(g4_ctx *ctx, const g4_kv *kv, int32_t layer, const float *d_q, float *
   a.scale = scale;
   a.window = window;
   a.sinks = sinks;
-  return launch_status(g4::launch_paged(a, ctx->dev, nullptr, ctx->stream), "paged attention");
+  Carve c;
+  const size_t o = c.add(g4::paged_scratch_bytes(a, ctx->dev));
+  G4_TRY(ensure_scratch(ctx, c.off));
+  return launch_status(g4::launch_paged(a, ctx->dev, ctx->scratch + o, ctx->stream), "paged attention");
 }
 
 }  // namespace

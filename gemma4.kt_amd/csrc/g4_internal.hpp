@@ -299,6 +299,7 @@ struct PagedArgs {
   int32_t window;  // 0: none
   int32_t sinks;
 };
+size_t paged_scratch_bytes(const PagedArgs &a, const DevInfo &dev);
 hipError_t launch_paged(const PagedArgs &a, const DevInfo &dev, char *scratch, hipStream_t s);
 
 }  // namespace g4
