@@ -1777,8 +1777,8 @@ int paged(g4_ctx *ctx, const g4_kv *kv, int32_t layer, const float *d_q, float *
     return fail(G4_ERR_INVALID_ARGUMENT, "%d heads over %d kv heads (a multiple, at most 1024)", n_heads,
                 kv->n_kv_heads);
   G4_TRY(check_list(n, d_seqs, d_seqs));
-  if (n_rows < 0 || (int64_t)n_rows * n_heads * kv->head_size > (int64_t(1) << 40))
-    return fail(G4_ERR_INVALID_ARGUMENT, "%d rows", n_rows);
+  if (n_rows < 0 || ((int64_t)n_rows + n) * n_heads > 0x7fffffff)
+    return fail(G4_ERR_INVALID_ARGUMENT, "%d rows of %d heads", n_rows, n_heads);
   if (window < 0 || sinks < 0) return fail(G4_ERR_INVALID_ARGUMENT, "window %d, first tokens %d", window, sinks);
   if (!(__builtin_fabsf(scale) <= 3.4028234663852886e38f)) return fail(G4_ERR_INVALID_ARGUMENT, "the scale is not finite");
   if (n == 0 || n_rows == 0) return G4_OK;
@@ -1801,8 +1801,10 @@ int paged(g4_ctx *ctx, const g4_kv *kv, int32_t layer, const float *d_q, float *
   a.window = window;
   a.sinks = sinks;
   Carve c;
-  const size_t o = c.add(g4::paged_scratch_bytes(a, ctx->dev));
+  const size_t o = c.add(d_row_begin ? g4::prompt_scratch_bytes(a, ctx->dev) : g4::paged_scratch_bytes(a, ctx->dev));
   G4_TRY(ensure_scratch(ctx, c.off));
+  if (d_row_begin)
+    return launch_status(g4::launch_prompt(a, ctx->dev, ctx->scratch + o, ctx->stream), "paged prompt attention");
   return launch_status(g4::launch_paged(a, ctx->dev, ctx->scratch + o, ctx->stream), "paged attention");
 }
 

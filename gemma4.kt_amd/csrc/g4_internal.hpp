@@ -300,6 +300,8 @@ struct PagedArgs {
   int32_t sinks;
 };
 size_t paged_scratch_bytes(const PagedArgs &a, const DevInfo &dev);
-hipError_t launch_paged(const PagedArgs &a, const DevInfo &dev, char *scratch, hipStream_t s);
+hipError_t launch_paged(const PagedArgs &a, const DevInfo &dev, char *scratch, hipStream_t s);  // row_begin null
+size_t prompt_scratch_bytes(const PagedArgs &a, const DevInfo &dev);
+hipError_t launch_prompt(const PagedArgs &a, const DevInfo &dev, char *scratch, hipStream_t s);
 
 }  // namespace g4

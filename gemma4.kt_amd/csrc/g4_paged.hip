@@ -1,212 +1,14 @@
-// g4_paged.hip -- attention over a paged key-value cache.
+// g4_paged.hip -- decode attention over a paged key-value cache.
 //
-// Row r of a call is token `pos` of a sequence; query head h reads kv head h / group.
-// It sees the tokens t <= pos of its sequence with t > pos - window (window > 0) or
-// t < sinks, and of those the ones whose page is there:
+// Row r of a call is the last token of a sequence; query head h reads kv head
+// h / group.  It sees the tokens t <= pos of its sequence with t > pos - window
+// (window > 0) or t < sinks, and of those the ones whose page is there:
 //   out = sum_t p_t V[t] / sum_t p_t,  p_t = exp(scale q . K[t] - max),
 // and zeros where it sees nothing.  One pass over K and V with a running maximum and
 // sum; products, statistics and sums are fp32 whatever the cache holds.
-#include "g4_device.hpp"
-#include "g4_internal.hpp"
+#include "g4_paged.hpp"
 
 namespace g4 {
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
-constexpr float LOG2E = 1.4426950408889634f;
-
-// What a row sees: visible index j < ns is token j, later ones are token j + skip.
-struct Seen {
-  int count;
-  int ns;
-  int skip;
-};
-
-G4_DEV Seen seen_by(int pos, int window, int sinks) {
-  Seen s;
-  const int from = window > 0 ? max(0, pos - window + 1) : 0;
-  s.ns = min(sinks, from);
-  s.skip = from - s.ns;
-  s.count = pos + 1 - s.skip;
-  return s;
-}
-
-G4_DEV bool page_ok(int page, const KvArgs &kv) { return (unsigned)page < (unsigned)kv.n_pages; }
-
-// Entry of row r in the list and its position; false where the row belongs to no
-// sequence (it is left as it is).  A position that its sequence does not have is -1.
-G4_DEV bool row_place(const PagedArgs &a, int r, int &seq, int &pos) {
-  int e = r, rows = 1, at = 0;
-  if (a.row_begin) {
-    if (r < a.row_begin[0] || r >= a.row_begin[a.n]) return false;
-    int lo = 0, hi = a.n - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (a.row_begin[mid] <= r) lo = mid;
-      else hi = mid - 1;
-    }
-    e = lo;
-    rows = a.row_begin[e + 1] - a.row_begin[e];
-    at = r - a.row_begin[e];
-  }
-  seq = a.seqs[e];
-  int len = 0;
-  if ((unsigned)seq < (unsigned)a.kv.max_seqs) len = min(max(a.kv.lengths[seq], 0), a.kv.max_pages << a.kv.shift);
-  else seq = 0;
-  pos = len - rows + at;
-  if (pos < 0 || pos >= len) pos = -1;
-  return true;
-}
-
-// Eight elements of a cached row as they are loaded, and as fp32.
-template <int TYPE>
-struct Raw8 {
-  u32x4 w[TYPE == T_F32 ? 2 : 1];
-  G4_DEV void load(const char *base, int64_t elem) {
-    const u32x4 *p = (const u32x4 *)(base + elem * (TYPE == T_F32 ? 4 : 2));
-#pragma unroll
-    for (int i = 0; i < (TYPE == T_F32 ? 2 : 1); ++i) w[i] = p[i];
-  }
-  G4_DEV void zero() {
-#pragma unroll
-    for (int i = 0; i < (TYPE == T_F32 ? 2 : 1); ++i) w[i] = u32x4{0, 0, 0, 0};
-  }
-  G4_DEV void floats(float (&f)[8]) const {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (TYPE == T_F32) f[i] = __uint_as_float(w[i >> 2][i & 3]);
-      else if constexpr (TYPE == T_F16) f[i] = i & 1 ? f16hi(w[0][i >> 1]) : f16lo(w[0][i >> 1]);
-      else f[i] = __uint_as_float(i & 1 ? w[0][i >> 1] & 0xFFFF0000u : w[0][i >> 1] << 16);
-    }
-  }
-};
-
-template <int N>
-G4_DEV float lanes_sum(float s, int lane) {  // over each aligned group of N lanes, in every lane of it
-  if constexpr (N > 1) s += __uint_as_float(partner_u32<1>(__float_as_uint(s), lane));
-  if constexpr (N > 2) s += __uint_as_float(partner_u32<2>(__float_as_uint(s), lane));
-  if constexpr (N > 4) s += __uint_as_float(partner_u32<4>(__float_as_uint(s), lane));
-  if constexpr (N > 8) s += __uint_as_float(partner_u32<8>(__float_as_uint(s), lane));
-  if constexpr (N > 16) s += __uint_as_float(partner_u32<16>(__float_as_uint(s), lane));
-  if constexpr (N > 32) s += __uint_as_float(partner_u32<32>(__float_as_uint(s), lane));
-  return s;
-}
-
-// 2^(a - b), b >= a, where both may be -infinity (nothing seen yet, or a hidden token)
-G4_DEV float shrink(float a, float b) { return a == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(a - b); }
-
-// One workgroup per (row, kv head, stretch of up to GT of its query heads).  LS = HS / 8
-// lanes share a cached row, eight elements a lane, so a wave takes RS = 64 / LS rows at
-// a time, U of them in flight.  Each group of LS lanes keeps a running maximum, sum and
-// accumulator of the rows it has met; the groups of the four waves are joined at the
-// end.  Head sizes between the powers of two leave the lanes behind the head idle.
-template <int TYPE, int HS, int GT>
-__global__ __launch_bounds__(256) void k_paged_row(PagedArgs a) {
-  constexpr int LS = HS / 8, RS = 64 / LS, U = 4;
-  __shared__ float sm[4 * RS][GT], sl[4 * RS][GT];
-  __shared__ float so[4][GT][HS];
-  const KvArgs &kv = a.kv;
-  if (*kv.status != KV_OK) return;
-  const int group = a.n_heads / kv.n_kv, parts = (group + GT - 1) / GT;
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, ql = lane % LS, rl = lane / LS;
-  const int kvh = blockIdx.y / parts, g0 = (blockIdx.y % parts) * GT;
-  int seq, pos;
-  if (!row_place(a, blockIdx.x, seq, pos)) return;
-  const Seen see = seen_by(pos, a.window, a.sinks);
-  const bool live = 8 * ql < kv.hs;
-  const int32_t *table = kv.table + (int64_t)seq * kv.max_pages;
-  const int64_t head_rows = ((int64_t)a.layer * kv.n_pages * kv.n_kv + kvh) << kv.shift;
-
-  float q[GT][8], acc[GT][8], m[GT], l[GT];
-  const float f = a.scale * LOG2E;
-#pragma unroll
-  for (int g = 0; g < GT; ++g) {
-    const int h = kvh * group + min(g0 + g, group - 1);
-    const float4 *qp = (const float4 *)(a.q + ((int64_t)blockIdx.x * a.n_heads + h) * kv.hs) + 2 * ql;
-    const float4 x = live ? qp[0] : make_float4(0, 0, 0, 0), y = live ? qp[1] : make_float4(0, 0, 0, 0);
-    q[g][0] = x.x, q[g][1] = x.y, q[g][2] = x.z, q[g][3] = x.w, q[g][4] = y.x, q[g][5] = y.y, q[g][6] = y.z, q[g][7] = y.w;
-    m[g] = -__builtin_inff(), l[g] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[g][i] = 0.f;
-  }
-
-  for (int j0 = wid * RS * U; j0 < see.count; j0 += 4 * RS * U) {
-    Raw8<TYPE> kr[U], vr[U];
-    bool ok[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = j0 + u * RS + rl;
-      const int t = j < see.ns ? j : j + see.skip;
-      const int page = j < see.count ? table[t >> kv.shift] : -1;
-      ok[u] = page_ok(page, kv);
-      kr[u].zero(), vr[u].zero();
-      if (ok[u] && live) {
-        const int64_t at = (head_rows + (((int64_t)page * kv.n_kv) << kv.shift) + (t & (kv.page - 1))) * kv.hs + 8 * ql;
-        kr[u].load(kv.k, at);
-        vr[u].load(kv.v, at);
-      }
-    }
-#pragma unroll
-    for (int g = 0; g < GT; ++g) {
-      float s[U], top = m[g];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float k[8], d = 0.f;
-        kr[u].floats(k);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d = __builtin_fmaf(q[g][i], k[i], d);
-        d = lanes_sum<LS>(d, lane) * f;  // by all lanes of the wave
-        s[u] = ok[u] ? d : -__builtin_inff();
-        top = fmaxf(top, s[u]);
-      }
-      const float c = shrink(m[g], top);
-      m[g] = top;
-      l[g] *= c;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) acc[g][i] *= c;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const float e = shrink(s[u], top);
-        float v[8];
-        vr[u].floats(v);
-        l[g] += e;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) acc[g][i] = __builtin_fmaf(e, v[i], acc[g][i]);
-      }
-    }
-  }
-
-  // join: first the groups of a wave, then the waves
-  if (ql == 0)
-#pragma unroll
-    for (int g = 0; g < GT; ++g) sm[wid * RS + rl][g] = m[g], sl[wid * RS + rl][g] = l[g];
-  __syncthreads();
-#pragma unroll
-  for (int g = 0; g < GT; ++g) {
-    float top = -__builtin_inff();
-    for (int i = 0; i < 4 * RS; ++i) top = fmaxf(top, sm[i][g]);
-    const float c = shrink(m[g], top);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float v = acc[g][i] * c;
-#pragma unroll
-      for (int d = LS; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
-      if (rl == 0) so[wid][g][8 * ql + i] = v;
-    }
-  }
-  __syncthreads();
-  for (int i = tid; i < GT * HS; i += 256) {
-    const int g = i / HS, d = i % HS;
-    if (d >= kv.hs || g0 + g >= group) continue;
-    float top = -__builtin_inff(), sum = 0.f;
-    for (int j = 0; j < 4 * RS; ++j) top = fmaxf(top, sm[j][g]);
-    for (int j = 0; j < 4 * RS; ++j) sum = __builtin_fmaf(sl[j][g], shrink(sm[j][g], top), sum);
-    const float o = ((so[0][g][d] + so[1][g][d]) + so[2][g][d]) + so[3][g][d];
-    a.out[((int64_t)blockIdx.x * a.n_heads + kvh * group + g0 + g) * kv.hs + d] = sum == 0.f ? 0.f : o / sum;
-  }
-}
 
 // ---------------------------------------------------------- one token, split ----
 //
@@ -223,8 +25,7 @@ __global__ __launch_bounds__(256) void k_paged_row(PagedArgs a) {
 // cache the query's three 16-bit parts, which add up to it exactly, for F32 the query
 // itself; the products are then exact (F32: rounded once), and a lane's sum over its
 // four rows of C is the score of (head lane / 16, key lane % 16).  The queries carry
-// scale * log2(e) and are brought to [1, 2) by a power of two, so that no part is
-// subnormal or too large.  Values are weighted by the vector unit in fp32, eight
+// scale * log2(e) (split_scale keeps their parts in range).  Values are weighted by the vector unit in fp32, eight
 // elements of a row per lane, with the weights handed over through the wave's own LDS.
 // While a tile is worked on, the next one's keys and values are on their way.
 
@@ -271,83 +72,6 @@ struct SplitPlan {
 G4_DEV int64_t stretch_of(int64_t total, int wgs) {
   const int64_t per = (total + wgs - 1) / wgs;
   return per < SPLIT_MIN ? SPLIT_MIN : per;
-}
-
-template <int TYPE>
-struct Mfma;
-template <>
-struct Mfma<T_F32> {
-  static constexpr int STEP = 16;  // dims of a step: 4 adjacent ones per lane
-  G4_DEV static f32x4 step(u32x4 a, u32x4 b, f32x4 c) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
-    return c;
-  }
-};
-template <>
-struct Mfma<T_F16> {
-  static constexpr int STEP = 32;  // 8 adjacent ones per lane
-  G4_DEV static f32x4 step(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  }
-};
-template <>
-struct Mfma<T_BF16> {
-  static constexpr int STEP = 32;
-  G4_DEV static f32x4 step(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-  }
-};
-
-// Two fp32 values' next 16-bit parts, in one word; the values become the remainders.
-// BF16 truncates: three parts hold the 24 bits of a finite value.  F16 rounds to
-// nearest, 11 bits and a sign a part, of values below 2 in size.
-template <int TYPE>
-G4_DEV uint32_t take_part(float &x, float &y) {
-  if constexpr (TYPE == T_BF16) {
-    const uint32_t a = __float_as_uint(x) & 0xFFFF0000u, b = __float_as_uint(y) & 0xFFFF0000u;
-    x -= __uint_as_float(a);
-    y -= __uint_as_float(b);
-    return (a >> 16) | b;
-  } else {
-    const _Float16 a = (_Float16)x, b = (_Float16)y;
-    x -= (float)a;
-    y -= (float)b;
-    return (uint32_t)__builtin_bit_cast(uint16_t, a) | (uint32_t)__builtin_bit_cast(uint16_t, b) << 16;
-  }
-}
-
-// The power of two that brings a value of this size to [1, 2), and its inverse; 1 for
-// zero, subnormal and infinite sizes.
-G4_DEV void unit_scale(float size, float &to, float &back) {
-  const uint32_t e = __float_as_uint(size) >> 23 & 255;
-  const bool plain = e > 0 && e < 254;
-  to = plain ? __uint_as_float((254u - e) << 23) : 1.f;
-  back = plain ? __uint_as_float(e << 23) : 1.f;
-}
-
-G4_DEV float lanes16_max(float v, int lane) {
-  v = fmaxf(v, __uint_as_float(partner_u32<1>(__float_as_uint(v), lane)));
-  v = fmaxf(v, __uint_as_float(partner_u32<2>(__float_as_uint(v), lane)));
-  v = fmaxf(v, __uint_as_float(partner_u32<4>(__float_as_uint(v), lane)));
-  return fmaxf(v, __uint_as_float(partner_u32<8>(__float_as_uint(v), lane)));
-}
-
-// An offset that is the same in all lanes, in scalar registers: loads then take a scalar
-// base and 32 bits of offset a lane.
-G4_DEV int64_t uniform(int64_t v) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
-  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)v >> 32));
-  return (int64_t)((uint64_t)hi << 32 | lo);
-}
-
-// Values that are formed here, before what follows: loads into the registers of their
-// operands would otherwise be moved ahead, and the operands copied.
-template <int N>
-G4_DEV void formed(float (&v)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i]));
 }
 
 // A score whose products or sums the matrix cores could not form (an infinite key times
@@ -486,7 +210,7 @@ __global__ __launch_bounds__(256, split_per_cu(TYPE, HS, GT)) void k_paged_split
       top = fmaxf(top, __uint_as_float(partner_u32<16>(__float_as_uint(top), lane)));
       top = fmaxf(top, __uint_as_float(partner_u32<32>(__float_as_uint(top), lane)));
       float to, bk;
-      unit_scale(top, to, bk);
+      split_scale<TYPE>(top, to, bk);
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] *= to;
       if (lane == 0) back[h] = bk;
@@ -839,44 +563,20 @@ static void launch_split(const PagedArgs &a, const SplitPlan &p, hipStream_t s) 
   else launch_split<TYPE, 512>(a, p, s);
 }
 
-template <int TYPE, int HS>
-static void launch_row(const PagedArgs &a, hipStream_t s) {
-  const int group = a.n_heads / a.kv.n_kv;
-  if (group == 1)
-    hipLaunchKernelGGL((k_paged_row<TYPE, HS, 1>), dim3(a.n_rows, a.kv.n_kv), dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL((k_paged_row<TYPE, HS, 2>), dim3(a.n_rows, a.kv.n_kv * ((group + 1) / 2)), dim3(256), 0, s, a);
-}
-
-template <int TYPE>
-static void launch_size(const PagedArgs &a, hipStream_t s) {
-  if (a.kv.hs <= 64) launch_row<TYPE, 64>(a, s);
-  else if (a.kv.hs <= 128) launch_row<TYPE, 128>(a, s);
-  else if (a.kv.hs <= 256) launch_row<TYPE, 256>(a, s);
-  else launch_row<TYPE, 512>(a, s);
-}
-
 size_t paged_scratch_bytes(const PagedArgs &a, const DevInfo &dev) {
-  if (a.row_begin) return 0;
   SplitPlan p;
   return split_layout(a, dev, nullptr, &p);
 }
 
 hipError_t launch_paged(const PagedArgs &a, const DevInfo &dev, char *scratch, hipStream_t s) {
-  if (!a.row_begin) {
-    SplitPlan p;
-    split_layout(a, dev, scratch, &p);
-    if (a.kv.type == T_F32) launch_split<T_F32>(a, p, s);
-    else if (a.kv.type == T_F16) launch_split<T_F16>(a, p, s);
-    else launch_split<T_BF16>(a, p, s);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k_paged_join, dim3(a.n * a.n_heads, (a.kv.hs + 63) / 64), dim3(256), 0, s, a, p);
-    return hipGetLastError();
-  }
-  if (a.kv.type == T_F32) launch_size<T_F32>(a, s);
-  else if (a.kv.type == T_F16) launch_size<T_F16>(a, s);
-  else launch_size<T_BF16>(a, s);
+  SplitPlan p;
+  split_layout(a, dev, scratch, &p);
+  if (a.kv.type == T_F32) launch_split<T_F32>(a, p, s);
+  else if (a.kv.type == T_F16) launch_split<T_F16>(a, p, s);
+  else launch_split<T_BF16>(a, p, s);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(k_paged_join, dim3(a.n * a.n_heads, (a.kv.hs + 63) / 64), dim3(256), 0, s, a, p);
   return hipGetLastError();
 }
 

@@ -1,0 +1,743 @@
+// g4_prompt.hip -- attention of several tokens per sequence over a paged key-value
+// cache: prompts, their chunks, drafted tokens.
+//
+// Every row is a token of a sequence and a query head; it sees what g4_paged.hip says,
+// causally.  A query tile is up to BM rows of one sequence that share a kv head: its
+// consecutive tokens times the heads of that kv head.  Keys and values come in tiles of
+// KT tokens through LDS (two buffers, loaded straight to LDS while the other is worked
+// on) and are used by all waves; a wave has 16 rows.
+//
+// Both products are on the matrix cores, transposed, so that a lane stays with one row
+// (column lane % 16 of every product):
+//   S^T = K Q^T   A = keys from LDS, B = the query's parts, which stay in registers
+//   O^T = V^T P^T A = values from LDS, read transposed, B = the weights: a lane's scores
+//                 are the weights it needs, since the keys of a product may come in any
+//                 order as long as A and B agree
+// For BF16 the queries and the weights are three bf16 parts each, exact; for F16 two
+// f16 parts (22 bits) of values scaled by a power of two; an F32 cache takes the fp32
+// products.  The running maximum and sum are fp32.  The matrix cores round every sum
+// down, so each tile's O^T is summed on its own, added in fp32, and every second tile
+// is computed with -P and subtracted: those errors then cancel instead of adding up.
+//
+// The (kv head, query tile, key tile) units are cut into equal stretches, one per
+// persistent workgroup, whatever the lengths, windows and causal triangles are
+// (k_prompt_plan counts them); a query tile whose key tiles are spread over several
+// stretches leaves (maximum, sum, O) of each in a slot, and k_prompt_join adds them.  A
+// row whose sums are not finite (an infinite or NaN key or value among those it meets,
+// maybe hidden from it) is computed again by k_prompt_join, from the formula.
+#include "g4_paged.hpp"
+
+namespace g4 {
+
+constexpr int PROMPT_MIN = 4;  // least key tiles of a stretch
+
+struct PromptPlan {
+  int32_t *n_tiles;  // query tiles, and the key tiles of all of them (as int64 behind it)
+  int64_t *total;
+  int64_t *first;    // [cap] key tiles before each query tile
+  int32_t *count;    // [cap] its key tiles
+  int32_t *entry;    // [cap] its sequence in the list
+  int32_t *tok;      // [cap] its first row's place in the sequence's rows
+  uint16_t *odd;     // [cap][units][BM / 16] rows whose sums are not finite
+  float *part;       // [2 * wgs][bm][hs]
+  float *ml;         // [2 * wgs][bm][2]
+  int32_t cap;
+  int32_t wgs;
+  int32_t bm;
+  int32_t kt;
+  int32_t gh;        // query heads of a tile
+  int32_t parts;     // head parts of a kv head
+  int32_t tt;        // tokens of a query tile
+};
+
+// Rows of entry e, inside the call's whatever row_begin holds.
+G4_DEV void entry_rows(const PagedArgs &a, int e, int &from, int &to) {
+  from = min(max(a.row_begin[e], 0), a.n_rows);
+  to = min(max(a.row_begin[e + 1], from), a.n_rows);
+}
+
+G4_DEV int entry_length(const PagedArgs &a, int e, int &seq) {
+  seq = a.seqs[e];
+  if ((unsigned)seq >= (unsigned)a.kv.max_seqs) {
+    seq = 0;
+    return 0;
+  }
+  return min(max(a.kv.lengths[seq], 0), a.kv.max_pages << a.kv.shift);
+}
+
+// The key tiles that positions p0 .. p1 see together: the first `st`, then those from a0.
+struct KeyTiles {
+  int count;
+  int st;
+  int a0;
+};
+
+G4_DEV KeyTiles key_tiles(int p0, int p1, int window, int sinks, int kt) {
+  KeyTiles k;
+  const int from = window > 0 ? max(0, max(p0, 0) - window + 1) : 0;
+  k.st = (min(sinks, from) + kt - 1) / kt;
+  k.a0 = max(from / kt, k.st);
+  k.count = p1 < 0 ? 0 : k.st + p1 / kt + 1 - k.a0;
+  return k;
+}
+
+// One workgroup: the query tiles of every sequence in order, and their key tiles.
+__global__ __launch_bounds__(1024) void k_prompt_plan(PagedArgs a, PromptPlan pl) {
+  __shared__ int tiles[1025], wsum[16];
+  __shared__ int64_t wsum64[16];
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  if (*a.kv.status != KV_OK) return;
+  int mine = 0;
+  if (tid < a.n) {
+    int from, to;
+    entry_rows(a, tid, from, to);
+    mine = (to - from + pl.tt - 1) / pl.tt;
+  }
+  int x = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(x, d, 64);
+    if (lane >= d) x += y;
+  }
+  if (lane == 63) wsum[wid] = x;
+  __syncthreads();
+  for (int w = 0; w < wid; ++w) x += wsum[w];
+  tiles[tid + 1] = x;
+  if (tid == 0) tiles[0] = 0;
+  __syncthreads();
+  const int n_tiles = min(tiles[a.n], pl.cap);
+  int64_t before = 0;
+  for (int t0 = 0; t0 < n_tiles; t0 += 1024) {
+    const int t = t0 + tid;
+    int count = 0;
+    if (t < n_tiles) {
+      int lo = 0, hi = a.n - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (tiles[mid] <= t) lo = mid;
+        else hi = mid - 1;
+      }
+      int from, to, seq;
+      entry_rows(a, lo, from, to);
+      const int rows = to - from, tok = (t - tiles[lo]) * pl.tt, len = entry_length(a, lo, seq);
+      const int p0 = len - rows + tok, p1 = min(p0 + pl.tt, len - rows + rows) - 1;
+      count = key_tiles(p0, p1, a.window, a.sinks, pl.kt).count;
+      pl.count[t] = count;
+      pl.entry[t] = lo;
+      pl.tok[t] = tok;
+    }
+    int64_t s = count;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t y = __shfl_up(s, d, 64);
+      if (lane >= d) s += y;
+    }
+    if (lane == 63) wsum64[wid] = s;
+    __syncthreads();
+    int64_t all = 0, mybase = before;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wid) mybase += wsum64[w];
+      all += wsum64[w];
+    }
+    if (t < n_tiles) pl.first[t] = mybase + s - count;
+    before += all;
+    __syncthreads();
+  }
+  if (tid == 0) *pl.n_tiles = n_tiles, *pl.total = before;
+}
+
+G4_DEV int64_t prompt_stretch(int64_t total, int wgs) {
+  const int64_t per = (total + wgs - 1) / wgs;
+  return per < PROMPT_MIN ? PROMPT_MIN : per;
+}
+
+// 16 bytes a lane from src (the same in all lanes) + off to LDS at `to` + 16 * lane.
+G4_DEV void load_to_lds(const char *src, uint32_t off, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(src)
+               : "memory", "m0");
+}
+
+// The loads to LDS and the LDS operations of the wave are done; then all waves meet.
+G4_DEV void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+constexpr int prompt_waves(int hs) { return hs > 256 ? 4 : 8; }
+constexpr int prompt_kt(int type, int hs) {
+  const int es = type == T_F32 ? 4 : 2, kt = 32768 / (hs * es);
+  return kt > 64 ? 64 : kt >= 64 ? 64 : kt >= 32 ? 32 : 16;
+}
+
+// The swizzles.  A row of LDS is CH = HS * ES / 16 words of 16 bytes, word c of row r
+// standing at c ^ k_swz(r) or c ^ v_swz(r).  16 keys' words at one c (an A operand of
+// S^T), and 8 rows' pairs of words (a transposed read of values), then lie on different
+// banks.  CH is an odd number times 2^z: only its low z bits may be changed.
+template <int CH>
+struct Swz {
+  static constexpr int Z = CH % 16 == 0 ? 4 : CH % 8 == 0 ? 3 : CH % 4 == 0 ? 2 : 0;
+  static_assert(Z > 0, "words of a row");
+  G4_DEV static int k(int row) { return (row & 15) >> (4 - Z); }
+  // pairs of words (16-bit values) or fours (fp32 values, rows 4 apart)
+  G4_DEV static int v16(int row) { return 2 * (((row & 15) >> (4 - Z)) & ((1 << (Z - 1)) - 1)); }
+  G4_DEV static int v32(int row) { return Z >= 4 ? 4 * ((row & 15) >> 2) : Z == 3 ? 4 * ((row & 7) >> 2) : 0; }
+};
+
+template <int TYPE, int HS>
+__global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k_paged_prompt(PagedArgs a,
+                                                                                             PromptPlan pl) {
+  using M = Mfma<TYPE>;
+  constexpr bool F32 = TYPE == T_F32;
+  constexpr int NW = prompt_waves(HS), BM = 16 * NW, KT = prompt_kt(TYPE, HS), ES = F32 ? 4 : 2;
+  constexpr int NP = TYPE == T_BF16 ? 3 : TYPE == T_F16 ? 2 : 1;  // parts of a query or weight
+  constexpr int STEPS = HS / M::STEP, NT = KT / 16, ND = HS / 16;
+  constexpr int CH = HS * ES / 16, ROW = HS * ES, GROUP = 16 * ROW, HALF = KT * ROW;
+  constexpr int IPW = 2 * KT * CH / 64 / NW, IPG = CH / 4;  // 1 KB loads of a wave, of a 16-token group
+  static_assert(IPW >= 1 && IPW * NW * 64 == 2 * KT * CH && (IPG % IPW == 0 || IPW % IPG == 0), "loads of a tile");
+  constexpr int UPW = IPW > IPG ? IPW / IPG : 1, IPU = IPW / UPW;  // groups (of keys or values) a wave loads, loads of each
+  using Z = Swz<CH>;
+  __shared__ __align__(1024) char lds[4 * HALF];  // [buffer][keys, values][KT][ROW]
+  __shared__ int32_t okf[2][NT];                  // the groups' pages are there
+
+  const KvArgs &kv = a.kv;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), hs = kv.hs;
+  if (*kv.status != KV_OK) return;
+  const int group = a.n_heads / kv.n_kv, units = kv.n_kv * pl.parts, n_tiles = *pl.n_tiles;
+  const int64_t per_unit = *pl.total, total = per_unit * units;
+
+  // rows that see nothing
+  for (int t = blockIdx.x; t < n_tiles; t += gridDim.x)
+    if (pl.count[t] == 0) {
+      int from, to;
+      entry_rows(a, pl.entry[t], from, to);
+      const int r0 = from + pl.tok[t], r1 = min(to, r0 + pl.tt);
+      for (int64_t i = (int64_t)r0 * a.n_heads * hs + tid; i < (int64_t)r1 * a.n_heads * hs; i += 64 * NW) a.out[i] = 0.f;
+    }
+
+  // Workgroups b, b + 8, ... run on one XCD: they take neighbouring stretches, so that
+  // the key tiles of a kv head are read into few L2s.
+  const int64_t per = prompt_stretch(total, pl.wgs);
+  const int stretch = pl.wgs % 8 == 0 ? (blockIdx.x & 7) * (pl.wgs >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+  const int64_t begin = stretch * per, end = min(total, begin + per);
+
+  const int col = lane & 15, g4 = lane >> 4;  // row of the tile's 16; quarter of a step, or of a key tile's 16
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+
+  // ---- where this lane's 16 bytes of each load come from, within a group's rows of a head
+  uint32_t src_off[IPW];
+#pragma unroll
+  for (int i = 0; i < IPW; ++i) {
+    const int unit = (wid * IPW + i) / IPG, at = (wid * IPW + i) % IPG * 64 + lane;
+    const int row = at / CH, c = at % CH, swz = unit < NT ? Z::k(row) : F32 ? Z::v32(row) : Z::v16(row);
+    src_off[i] = (uint32_t)(row * hs * ES + min((c ^ swz) * 16, hs * ES - 16));
+  }
+  const int64_t layer_rows = (int64_t)a.layer * kv.n_pages * kv.n_kv << kv.shift;
+
+  for (int64_t u = begin; u < end;) {
+    const int hu = (int)(u / per_unit);
+    const int64_t rel = u - hu * per_unit;
+    int tile;
+    {
+      int lo = 0, hi = n_tiles - 1;  // the last tile whose first key tile is <= rel
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (pl.first[mid] <= rel) lo = mid;
+        else hi = mid - 1;
+      }
+      tile = __builtin_amdgcn_readfirstlane(lo);
+    }
+    const int cnt = __builtin_amdgcn_readfirstlane(pl.count[tile]);
+    const int j0 = __builtin_amdgcn_readfirstlane((int)(rel - pl.first[tile]));
+    const int j1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)cnt, j0 + (end - u)));
+    const int kvh = __builtin_amdgcn_readfirstlane(hu / pl.parts);
+    const int h0 = (hu - kvh * pl.parts) * pl.gh, heads = min(pl.gh, group - h0);
+    const int e = __builtin_amdgcn_readfirstlane(pl.entry[tile]), tok0 = __builtin_amdgcn_readfirstlane(pl.tok[tile]);
+    int from, to, seq;
+    entry_rows(a, e, from, to);
+    const int len = __builtin_amdgcn_readfirstlane(entry_length(a, e, seq));
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    const int base = len - (to - from) + tok0;  // position of the tile's first row
+    const int toks = min(pl.tt, to - from - tok0);
+    const KeyTiles kts = key_tiles(base, base + toks - 1, a.window, a.sinks, KT);
+    const int32_t *table = kv.table + (int64_t)seq * kv.max_pages;
+
+    // ---- this lane's row
+    const int r = wid * 16 + col, tk = r / heads, hd = r - tk * heads;
+    const bool row_ok = tk < toks;
+    const int pos = row_ok ? base + tk : -1;
+    const int seen_from = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    const int first_tk = wid * 16 / heads, last_tk = min((wid * 16 + 15) / heads, toks - 1);
+    const bool wave_on = first_tk < toks && base + last_tk >= 0;  // uniform
+    const int wave_lo = base + first_tk, wave_hi = base + last_tk;
+    const int wave_from0 = a.window > 0 ? max(0, max(wave_lo, 0) - a.window + 1) : 0;
+    const int wave_from = a.window > 0 ? max(0, wave_hi - a.window + 1) : 0;
+    const int64_t q_row = ((int64_t)(from + tok0 + tk) * a.n_heads + kvh * group + h0 + hd) * hs;
+
+    // ---- the query's parts, as B operands
+    u32x4 qb[NP][STEPS];
+    float back;
+    {
+      const float f = a.scale * LOG2E;
+      constexpr int W = F32 ? 4 : 8;
+      float x[STEPS][W], top = 0.f;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        const int d = s * M::STEP + g4 * W;
+        const bool in = row_ok && d < hs;
+#pragma unroll
+        for (int i = 0; i < W; i += 4) {
+          const float4 v = in ? *(const float4 *)(a.q + q_row + d + i) : make_float4(0, 0, 0, 0);
+          x[s][i] = v.x * f, x[s][i + 1] = v.y * f, x[s][i + 2] = v.z * f, x[s][i + 3] = v.w * f;
+        }
+#pragma unroll
+        for (int i = 0; i < W; ++i) top = fmaxf(top, __builtin_fabsf(x[s][i]));
+      }
+      top = fmaxf(top, __uint_as_float(partner_u32<16>(__float_as_uint(top), lane)));
+      top = fmaxf(top, __uint_as_float(partner_u32<32>(__float_as_uint(top), lane)));
+      float scale_to;
+      split_scale<TYPE>(top, scale_to, back);
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) x[s][i] *= scale_to;
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (F32) qb[p][s][i] = __float_as_uint(x[s][i]);
+            else qb[p][s][i] = take_part<TYPE>(x[s][2 * i], x[s][2 * i + 1]);
+          }
+      }
+    }
+
+    f32x4 o[ND];  // the sums so far times the last tile's sign
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -__builtin_inff(), l = 0.f;
+    float sign = 1.f;
+
+    // ---- loads of key tile j to a buffer: this wave's groups
+    auto tile_token = [&](int j) { return (j < kts.st ? j : j - kts.st + kts.a0) * KT; };
+    auto page_at = [&](int j, int w) {  // the page of the wave's w-th group in tile j, -1 where there is none
+      const int gi = (wid * IPW / IPG + w) % NT, t = tile_token(j) + gi * 16;
+      const bool in = j < j1 && t < len;
+      const int page = table[in ? t >> kv.shift : 0];
+      return in && page_ok(page, kv) ? page : -1;
+    };
+    auto issue = [&](int j, int buf, const int (&pages)[UPW]) {
+#pragma unroll
+      for (int w = 0; w < UPW; ++w) {
+        const int unit = wid * IPW / IPG + w, gi = unit % NT, t = tile_token(j) + gi * 16;
+        const bool values = unit >= NT;
+        const int page = __builtin_amdgcn_readfirstlane(pages[w]);
+        const char *src = (values ? kv.v : kv.k) +
+                          uniform((layer_rows + (((int64_t)max(page, 0) * kv.n_kv + kvh) << kv.shift) + (t & (kv.page - 1))) *
+                                  (int64_t)(hs * ES));
+        const int first = wid * IPW % IPG;  // load of the group this wave begins with
+        const uint32_t to_off = buf * 2 * HALF + (values ? HALF : 0) + gi * GROUP + first * 1024;
+        if (!values && first == 0 && lane == 0) okf[buf][gi] = page >= 0;
+        if (values && (page < 0 || t + 16 > len)) {
+          // rows that hold no token: zeros, since a weight of zero does not silence a NaN
+#pragma unroll
+          for (int i = 0; i < IPU; ++i) {
+            const int row = ((first + i) * 64 + lane) / CH;
+            u32x4 v = *(const u32x4 *)(src + src_off[w * IPU + i]);
+            const bool in = page >= 0 && t + row < len;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) v[x] = in ? v[x] : 0u;
+            *(u32x4 *)(lds + to_off + i * 1024 + lane * 16) = v;
+          }
+        } else if (page >= 0) {
+#pragma unroll
+          for (int i = 0; i < IPU; ++i) load_to_lds(src, src_off[w * IPU + i], lds0 + to_off + i * 1024);
+        }
+      }
+    };
+
+    int pages[UPW];
+#pragma unroll
+    for (int w = 0; w < UPW; ++w) pages[w] = page_at(j0, w);
+    tile_barrier();  // the last segment's tiles are done with
+    issue(j0, 0, pages);
+#pragma unroll
+    for (int w = 0; w < UPW; ++w) pages[w] = page_at(j0 + 1, w);
+
+    for (int j = j0; j < j1; ++j) {
+      const int buf = (j - j0) & 1, t0 = tile_token(j);
+      tile_barrier();  // tile j is here, and everyone is done with tile j - 1
+      if (j + 1 < j1) {
+        issue(j + 1, buf ^ 1, pages);
+#pragma unroll
+        for (int w = 0; w < UPW; ++w) pages[w] = page_at(j + 2, w);
+      }
+      if (!wave_on || t0 > wave_hi || (t0 + KT <= wave_from0 && t0 >= a.sinks)) continue;  // nothing seen
+      const char *kt_lds = lds + buf * 2 * HALF, *vt_lds = kt_lds + HALF;
+
+      // ---- scores of the tile: s[n][i] of key 16 n + 4 g4 + i
+      f32x4 s[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+      {
+        const int x = g4 ^ Z::k(col);
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const u32x4 k = *(const u32x4 *)(kt_lds + (n * 16 + col) * ROW + (((4 * st) ^ x) << 4));
+#pragma unroll
+            for (int p = NP - 1; p >= 0; --p) s[n] = M::step(k, qb[p][st], s[n]);
+          }
+      }
+
+      // ---- what the row sees of them
+      bool all_pages = true;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) all_pages &= __builtin_amdgcn_readfirstlane(okf[buf][n]) != 0;
+      const bool full = all_pages && t0 + KT - 1 <= wave_lo && (t0 >= wave_from || t0 + KT - 1 < a.sinks);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] *= back;
+      if (!full) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const bool there = okf[buf][n] != 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int t = t0 + n * 16 + 4 * g4 + i;
+            const bool seen = there && t <= pos && (t >= seen_from || t < a.sinks);
+            s[n][i] = seen ? s[n][i] : -__builtin_inff();
+          }
+        }
+      }
+
+      // ---- weights
+      float top = s[0][0];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[n][i]);
+      top = fmaxf(top, __uint_as_float(partner_u32<16>(__float_as_uint(top), lane)));
+      top = fmaxf(top, __uint_as_float(partner_u32<32>(__float_as_uint(top), lane)));
+      top = fmaxf(m, top);
+      // weights of F16 stand 2^14 higher, so that the second part of a small one is not subnormal
+      const float up = TYPE == T_F16 ? 14.f : 0.f;
+      const float zero = top == -__builtin_inff() ? 0.f : top - up;
+      const float shrunk = __builtin_amdgcn_exp2f(m - (zero + up));
+      m = top;
+      float sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float w = __builtin_amdgcn_exp2f(s[n][i] - zero);
+          sum += w;
+          s[n][i] = w * sign;
+        }
+      l = __builtin_fmaf(l, shrunk, sum);
+
+      // ---- O^T = shrunk O^T + V^T P^T
+      if constexpr (F32) {
+        const int vx = Z::v32(4 * g4);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          f32x4 t = {0.f, 0.f, 0.f, 0.f};
+          const int word = ((4 * d) ^ vx) + (col >> 2);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float v = *(const float *)(vt_lds + (n * 16 + 4 * g4 + i) * ROW + word * 16 + 4 * (col & 3));
+              t = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s[n][i], t, 0, 0, 0);
+            }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[d][i] = __builtin_fmaf(o[d][i], -shrunk, t[i]);
+        }
+      } else {
+        u32x4 pb[NP][NT / 2];
+#pragma unroll
+        for (int n = 0; n < NT / 2; ++n)
+#pragma unroll
+          for (int p = 0; p < NP; ++p)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int k = 2 * n + (i >> 1), x = 2 * (i & 1);
+              float w0 = s[k][x], w1 = s[k][x + 1];
+              pb[p][n][i] = take_part<TYPE>(w0, w1);
+              s[k][x] = w0, s[k][x + 1] = w1;
+            }
+        const int row = 4 * g4 + (col >> 2), vx = ((col & 3) >> 1) ^ Z::v16(row);
+        const uint32_t v_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)vt_lds + row * ROW +
+                              8 * (col & 1);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          f32x4 t = {0.f, 0.f, 0.f, 0.f};
+          const uint32_t at = v_at + (((2 * d) ^ vx) << 4);
+#pragma unroll
+          for (int n = 0; n < NT / 2; ++n) {
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s16x4 *tr;
+            union {
+              s16x4 h[2];
+              u32x4 w;
+            } v;
+            v.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr)(uintptr_t)(at + (2 * n) * GROUP));
+            v.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr)(uintptr_t)(at + (2 * n + 1) * GROUP));
+#pragma unroll
+            for (int p = NP - 1; p >= 0; --p) t = M::step(v.w, pb[p][n], t);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[d][i] = __builtin_fmaf(o[d][i], -shrunk, t[i]);
+        }
+      }
+      sign = -sign;
+    }
+
+    // ---- the segment's result
+    l += __uint_as_float(partner_u32<16>(__float_as_uint(l), lane));
+    l += __uint_as_float(partner_u32<32>(__float_as_uint(l), lane));
+    const bool whole = j0 == 0 && j1 == cnt;
+    if (wave_on || first_tk < toks) {
+      const float fix = -sign;  // the last tile's sign
+      if (whole) {
+        const float inv = l == 0.f ? 0.f : fix / l;
+        bool odd = !(l < __builtin_inff());
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const int at = d * 16 + 4 * g4;
+          const float4 v = l == 0.f ? make_float4(0, 0, 0, 0)
+                                    : make_float4(o[d][0] * inv, o[d][1] * inv, o[d][2] * inv, o[d][3] * inv);
+          if (row_ok && at < hs) {
+            *(float4 *)(a.out + q_row + at) = v;
+            odd |= !(__builtin_fabsf(v.x) < __builtin_inff()) || !(__builtin_fabsf(v.y) < __builtin_inff()) ||
+                   !(__builtin_fabsf(v.z) < __builtin_inff()) || !(__builtin_fabsf(v.w) < __builtin_inff());
+          }
+        }
+        const uint64_t b = __ballot(odd && row_ok);
+        if (lane == 0)
+          pl.odd[((int64_t)tile * units + hu) * NW + wid] = (uint16_t)(b | b >> 16 | b >> 32 | b >> 48);
+      } else {
+        const int64_t slot = 2 * (int64_t)stretch + (u != begin);
+        float *part = pl.part + (slot * BM + r) * hs;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const int at = d * 16 + 4 * g4;
+          if (row_ok && at < hs) *(float4 *)(part + at) = make_float4(o[d][0] * fix, o[d][1] * fix, o[d][2] * fix, o[d][3] * fix);
+        }
+        if (g4 == 0 && row_ok) pl.ml[(slot * BM + r) * 2] = m, pl.ml[(slot * BM + r) * 2 + 1] = l;
+      }
+    }
+    u += j1 - j0;
+  }
+}
+
+// One row from the formula, by a workgroup of four waves: LS lanes share a cached row,
+// eight elements a lane, so a wave takes RS rows at a time, U of them in flight.  Each
+// group of LS lanes keeps a running maximum, sum and accumulator of the rows it has
+// met; they are joined at the end.
+template <int TYPE, int HS>
+G4_DEV void plain_row(const PagedArgs &a, int64_t out_row, int head, int seq, int pos, float *sm, float *sl, float *so) {
+  constexpr int LS = HS / 8, RS = 64 / LS, U = 4;
+  const KvArgs &kv = a.kv;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, ql = lane % LS, rl = lane / LS;
+  const int kvh = head / (a.n_heads / kv.n_kv);
+  const Seen see = seen_by(pos, a.window, a.sinks);
+  const bool live = 8 * ql < kv.hs;
+  const int32_t *table = kv.table + (int64_t)seq * kv.max_pages;
+  const int64_t head_rows = ((int64_t)a.layer * kv.n_pages * kv.n_kv + kvh) << kv.shift;
+  float q[8], acc[8], m = -__builtin_inff(), l = 0.f;
+  const float f = a.scale * LOG2E;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    q[i] = live ? a.q[(out_row * a.n_heads + head) * kv.hs + 8 * ql + i] : 0.f;
+    acc[i] = 0.f;
+  }
+  for (int j0 = wid * RS * U; j0 < see.count; j0 += 4 * RS * U) {
+    Raw8<TYPE> kr[U], vr[U];
+    bool ok[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * RS + rl;
+      const int t = j < see.ns ? j : j + see.skip;
+      const int page = j < see.count ? table[t >> kv.shift] : -1;
+      ok[u] = page_ok(page, kv);
+      kr[u].zero(), vr[u].zero();
+      if (ok[u] && live) {
+        const int64_t at = (head_rows + (((int64_t)page * kv.n_kv) << kv.shift) + (t & (kv.page - 1))) * kv.hs + 8 * ql;
+        kr[u].load(kv.k, at);
+        vr[u].load(kv.v, at);
+      }
+    }
+    float s[U], top = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float k[8], d = 0.f;
+      kr[u].floats(k);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) d = __builtin_fmaf(q[i], k[i], d);
+      d = lanes_sum<LS>(d, lane) * f;  // by all lanes of the wave
+      s[u] = ok[u] ? d : -__builtin_inff();
+      top = fmaxf(top, s[u]);
+    }
+    const float c = shrink(m, top);
+    m = top;
+    l *= c;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] *= c;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float e = shrink(s[u], top);
+      float v[8];
+      vr[u].floats(v);
+      l += e;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] = __builtin_fmaf(e, v[i], acc[i]);
+    }
+  }
+  __syncthreads();
+  if (ql == 0) sm[wid * RS + rl] = m, sl[wid * RS + rl] = l;
+  __syncthreads();
+  float top = -__builtin_inff(), sum = 0.f;
+  for (int i = 0; i < 4 * RS; ++i) top = fmaxf(top, sm[i]);
+  for (int i = 0; i < 4 * RS; ++i) sum = __builtin_fmaf(sl[i], shrink(sm[i], top), sum);
+  const float c = shrink(m, top);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float v = acc[i] * c;
+#pragma unroll
+    for (int d = LS; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
+    if (rl == 0) so[wid * HS + 8 * ql + i] = v;
+  }
+  __syncthreads();
+  for (int d = tid; d < kv.hs; d += 256) {
+    const float o = ((so[d] + so[HS + d]) + so[2 * HS + d]) + so[3 * HS + d];
+    a.out[(out_row * a.n_heads + head) * kv.hs + d] = sum == 0.f ? 0.f : o / sum;
+  }
+}
+
+// One workgroup per (query tile, kv head part): adds the slots of a tile whose key tiles
+// were spread over several stretches, in order, and computes rows again that are not finite.
+template <int TYPE, int HS>
+__global__ __launch_bounds__(256) void k_paged_prompt_join(PagedArgs a, PromptPlan pl) {
+  __shared__ float sm[4 * 8], sl[4 * 8], so[4 * HS];
+  __shared__ int32_t bad[128];
+  const KvArgs &kv = a.kv;
+  const int tid = threadIdx.x, hs = kv.hs;
+  if (*kv.status != KV_OK) return;
+  const int units = kv.n_kv * pl.parts, tile = blockIdx.x / units, hu = blockIdx.x - tile * units;
+  if (tile >= *pl.n_tiles) return;
+  const int cnt = pl.count[tile];
+  if (cnt == 0) return;
+  const int64_t per_unit = *pl.total, per = prompt_stretch(per_unit * units, pl.wgs);
+  const int64_t ua = hu * per_unit + pl.first[tile];
+  const int w0 = (int)(ua / per), w1 = (int)((ua + cnt - 1) / per);
+  const int group = a.n_heads / kv.n_kv, kvh = hu / pl.parts, h0 = (hu - kvh * pl.parts) * pl.gh;
+  const int heads = min(pl.gh, group - h0), e = pl.entry[tile], tok0 = pl.tok[tile];
+  int from, to, seq;
+  entry_rows(a, e, from, to);
+  const int len = entry_length(a, e, seq), rows = min(pl.tt, to - from - tok0) * heads;
+  if (tid < 128) bad[tid] = 0;
+  __syncthreads();
+  if (w0 != w1) {
+    const int64_t s0 = 2 * (int64_t)w0 + (ua != w0 * per);
+    const int words = hs / 4;
+    for (int i = tid; i < rows * words; i += 256) {
+      const int r = i / words, x = i - r * words;
+      float top = -__builtin_inff();
+      for (int w = w0; w <= w1; ++w) top = fmaxf(top, pl.ml[((w == w0 ? s0 : 2 * (int64_t)w) * pl.bm + r) * 2]);
+      float4 o = make_float4(0, 0, 0, 0);
+      float sum = 0.f;
+#pragma unroll 4
+      for (int w = w0; w <= w1; ++w) {
+        const int64_t at = (w == w0 ? s0 : 2 * (int64_t)w) * pl.bm + r;
+        const float c = shrink(pl.ml[at * 2], top);
+        const float4 v = *(const float4 *)(pl.part + at * hs + 4 * x);
+        sum = __builtin_fmaf(pl.ml[at * 2 + 1], c, sum);
+        o.x = __builtin_fmaf(v.x, c, o.x), o.y = __builtin_fmaf(v.y, c, o.y);
+        o.z = __builtin_fmaf(v.z, c, o.z), o.w = __builtin_fmaf(v.w, c, o.w);
+      }
+      const bool none = sum == 0.f;
+      o.x = none ? 0.f : o.x / sum, o.y = none ? 0.f : o.y / sum, o.z = none ? 0.f : o.z / sum, o.w = none ? 0.f : o.w / sum;
+      const int tk = r / heads, hd = r - tk * heads;
+      *(float4 *)(a.out + ((int64_t)(from + tok0 + tk) * a.n_heads + kvh * group + h0 + hd) * hs + 4 * x) = o;
+      if (!(__builtin_fabsf(o.x) < __builtin_inff()) || !(__builtin_fabsf(o.y) < __builtin_inff()) ||
+          !(__builtin_fabsf(o.z) < __builtin_inff()) || !(__builtin_fabsf(o.w) < __builtin_inff()))
+        bad[r] = 1;
+    }
+  } else if (tid < rows) {
+    bad[tid] = pl.odd[(int64_t)blockIdx.x * (pl.bm / 16) + (tid >> 4)] >> (tid & 15) & 1;
+  }
+  if (!__syncthreads_or(tid < 128 && bad[tid])) return;
+  for (int r = 0; r < rows; ++r) {
+    if (!bad[r]) continue;
+    const int tk = r / heads, hd = r - tk * heads;
+    plain_row<TYPE, HS>(a, from + tok0 + tk, kvh * group + h0 + hd, seq, len - (to - from) + tok0 + tk, sm, sl, so);
+  }
+}
+
+static int prompt_class(int hs) { return hs <= 64 ? 64 : hs <= 96 ? 96 : hs <= 128 ? 128 : hs <= 192 ? 192 : hs <= 256 ? 256 : 512; }
+
+static size_t prompt_layout(const PagedArgs &a, const DevInfo &dev, char *base, PromptPlan *p) {
+  const int hs = prompt_class(a.kv.hs), group = a.n_heads / a.kv.n_kv;
+  p->bm = 16 * prompt_waves(hs);
+  p->kt = prompt_kt(a.kv.type, hs);
+  p->gh = group < p->bm ? group : p->bm;
+  p->parts = (group + p->gh - 1) / p->gh;
+  p->tt = p->bm / p->gh;
+  p->wgs = dev.cu_count;
+  p->cap = a.n_rows / p->tt + a.n;
+  size_t off = 0;
+  auto add = [&](size_t bytes) {
+    char *at = base + off;
+    off += (bytes + 255) & ~size_t(255);
+    return at;
+  };
+  const size_t cap = (size_t)p->cap, units = (size_t)a.kv.n_kv * p->parts;
+  p->n_tiles = (int32_t *)add(4);
+  p->total = (int64_t *)add(8);
+  p->first = (int64_t *)add(8 * cap);
+  p->count = (int32_t *)add(4 * cap);
+  p->entry = (int32_t *)add(4 * cap);
+  p->tok = (int32_t *)add(4 * cap);
+  p->odd = (uint16_t *)add(2 * cap * units * (p->bm / 16));
+  p->part = (float *)add(sizeof(float) * 2 * (size_t)p->wgs * p->bm * a.kv.hs);
+  p->ml = (float *)add(sizeof(float) * 4 * (size_t)p->wgs * p->bm);
+  return off;
+}
+
+size_t prompt_scratch_bytes(const PagedArgs &a, const DevInfo &dev) {
+  PromptPlan p;
+  return prompt_layout(a, dev, nullptr, &p);
+}
+
+template <int TYPE, int HS>
+static hipError_t launch_tiles(const PagedArgs &a, const PromptPlan &p, hipStream_t s) {
+  hipLaunchKernelGGL((k_paged_prompt<TYPE, HS>), dim3(p.wgs), dim3(64 * prompt_waves(HS)), 0, s, a, p);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  constexpr int JHS = HS == 96 ? 128 : HS == 192 ? 256 : HS;
+  hipLaunchKernelGGL((k_paged_prompt_join<TYPE, JHS>), dim3(p.cap * a.kv.n_kv * p.parts), dim3(256), 0, s, a, p);
+  return hipGetLastError();
+}
+
+template <int TYPE>
+static hipError_t launch_tiles(const PagedArgs &a, const PromptPlan &p, hipStream_t s) {
+  switch (prompt_class(a.kv.hs)) {
+    case 64: return launch_tiles<TYPE, 64>(a, p, s);
+    case 96: return launch_tiles<TYPE, 96>(a, p, s);
+    case 128: return launch_tiles<TYPE, 128>(a, p, s);
+    case 192: return launch_tiles<TYPE, 192>(a, p, s);
+    case 256: return launch_tiles<TYPE, 256>(a, p, s);
+    default: return launch_tiles<TYPE, 512>(a, p, s);
+  }
+}
+
+hipError_t launch_prompt(const PagedArgs &a, const DevInfo &dev, char *scratch, hipStream_t s) {
+  PromptPlan p;
+  prompt_layout(a, dev, scratch, &p);
+  hipLaunchKernelGGL(k_prompt_plan, dim3(1), dim3(1024), 0, s, a, p);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  if (a.kv.type == T_F32) return launch_tiles<T_F32>(a, p, s);
+  if (a.kv.type == T_F16) return launch_tiles<T_F16>(a, p, s);
+  return launch_tiles<T_BF16>(a, p, s);
+}
+
+}  // namespace g4
