@@ -31,31 +31,6 @@ G4_DEV Seen seen_by(int pos, int window, int sinks) {
 
 G4_DEV bool page_ok(int page, const KvArgs &kv) { return (unsigned)page < (unsigned)kv.n_pages; }
 
-// Entry of row r in the list and its position; false where the row belongs to no
-// sequence (it is left as it is).  A position that its sequence does not have is -1.
-G4_DEV bool row_place(const PagedArgs &a, int r, int &seq, int &pos) {
-  int e = r, rows = 1, at = 0;
-  if (a.row_begin) {
-    if (r < a.row_begin[0] || r >= a.row_begin[a.n]) return false;
-    int lo = 0, hi = a.n - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (a.row_begin[mid] <= r) lo = mid;
-      else hi = mid - 1;
-    }
-    e = lo;
-    rows = a.row_begin[e + 1] - a.row_begin[e];
-    at = r - a.row_begin[e];
-  }
-  seq = a.seqs[e];
-  int len = 0;
-  if ((unsigned)seq < (unsigned)a.kv.max_seqs) len = min(max(a.kv.lengths[seq], 0), a.kv.max_pages << a.kv.shift);
-  else seq = 0;
-  pos = len - rows + at;
-  if (pos < 0 || pos >= len) pos = -1;
-  return true;
-}
-
 // Eight elements of a cached row as they are loaded, and as fp32.
 template <int TYPE>
 struct Raw8 {

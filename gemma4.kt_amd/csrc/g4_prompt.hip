@@ -29,25 +29,33 @@
 
 namespace g4 {
 
-constexpr int PROMPT_MIN = 4;  // least key tiles of a stretch
+// A query tile: rows row .. row + toks - 1 of the call, the first at position `base`, of a
+// sequence with `len` tokens; `count` key tiles, `first` of them before its own.
+struct PromptTile {
+  int32_t row;
+  int32_t toks;
+  int32_t base;
+  int32_t seq;
+  int32_t len;
+  int32_t count;
+  int64_t first;
+};
 
 struct PromptPlan {
-  int32_t *n_tiles;  // query tiles, and the key tiles of all of them (as int64 behind it)
-  int64_t *total;
-  int64_t *first;    // [cap] key tiles before each query tile
-  int32_t *count;    // [cap] its key tiles
-  int32_t *entry;    // [cap] its sequence in the list
-  int32_t *tok;      // [cap] its first row's place in the sequence's rows
-  uint16_t *odd;     // [cap][units][BM / 16] rows whose sums are not finite
-  float *part;       // [2 * wgs][bm][hs]
-  float *ml;         // [2 * wgs][bm][2]
+  int32_t *n_tiles;   // query tiles of a kv head part
+  int64_t *total;     // their key tiles
+  int32_t *start;     // [wgs] the query tile that a stretch begins in
+  PromptTile *tiles;  // [cap]
+  uint16_t *odd;      // [cap][units][bm / 16] rows whose sums are not finite
+  float *part;        // [2 * wgs][bm][hs]
+  float *ml;          // [2 * wgs][bm][2]
   int32_t cap;
   int32_t wgs;
   int32_t bm;
   int32_t kt;
-  int32_t gh;        // query heads of a tile
-  int32_t parts;     // head parts of a kv head
-  int32_t tt;        // tokens of a query tile
+  int32_t gh;         // query heads of a tile
+  int32_t parts;      // head parts of a kv head
+  int32_t tt;         // tokens of a query tile
 };
 
 // Rows of entry e, inside the call's whatever row_begin holds.
@@ -56,6 +64,7 @@ G4_DEV void entry_rows(const PagedArgs &a, int e, int &from, int &to) {
   to = min(max(a.row_begin[e + 1], from), a.n_rows);
 }
 
+// Length and number of its sequence.
 G4_DEV int entry_length(const PagedArgs &a, int e, int &seq) {
   seq = a.seqs[e];
   if ((unsigned)seq >= (unsigned)a.kv.max_seqs) {
@@ -81,7 +90,25 @@ G4_DEV KeyTiles key_tiles(int p0, int p1, int window, int sinks, int kt) {
   return k;
 }
 
-// One workgroup: the query tiles of every sequence in order, and their key tiles.
+// Key tiles of a stretch.
+G4_DEV int64_t prompt_stretch(int64_t total, int wgs) {
+  const int64_t per = (total + wgs - 1) / wgs;
+  return per < 1 ? 1 : per;
+}
+
+// The last tile whose first key tile is <= rel.
+G4_DEV int find_tile(const PromptTile *tiles, int n, int64_t rel) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (tiles[mid].first <= rel) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// One workgroup: the query tiles of every sequence in order, with their key tiles, and
+// the tile that each stretch begins in.
 __global__ __launch_bounds__(1024) void k_prompt_plan(PagedArgs a, PromptPlan pl) {
   __shared__ int tiles[1025], wsum[16];
   __shared__ int64_t wsum64[16];
@@ -109,7 +136,7 @@ __global__ __launch_bounds__(1024) void k_prompt_plan(PagedArgs a, PromptPlan pl
   int64_t before = 0;
   for (int t0 = 0; t0 < n_tiles; t0 += 1024) {
     const int t = t0 + tid;
-    int count = 0;
+    PromptTile it = {};
     if (t < n_tiles) {
       int lo = 0, hi = a.n - 1;
       while (lo < hi) {
@@ -117,16 +144,16 @@ __global__ __launch_bounds__(1024) void k_prompt_plan(PagedArgs a, PromptPlan pl
         if (tiles[mid] <= t) lo = mid;
         else hi = mid - 1;
       }
-      int from, to, seq;
+      int from, to;
       entry_rows(a, lo, from, to);
-      const int rows = to - from, tok = (t - tiles[lo]) * pl.tt, len = entry_length(a, lo, seq);
-      const int p0 = len - rows + tok, p1 = min(p0 + pl.tt, len - rows + rows) - 1;
-      count = key_tiles(p0, p1, a.window, a.sinks, pl.kt).count;
-      pl.count[t] = count;
-      pl.entry[t] = lo;
-      pl.tok[t] = tok;
+      const int tok = (t - tiles[lo]) * pl.tt;
+      it.len = entry_length(a, lo, it.seq);
+      it.row = from + tok;
+      it.toks = min(pl.tt, to - it.row);
+      it.base = it.len - (to - from) + tok;
+      it.count = key_tiles(it.base, it.base + it.toks - 1, a.window, a.sinks, pl.kt).count;
     }
-    int64_t s = count;
+    int64_t s = it.count;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int64_t y = __shfl_up(s, d, 64);
@@ -139,16 +166,20 @@ __global__ __launch_bounds__(1024) void k_prompt_plan(PagedArgs a, PromptPlan pl
       if (w < wid) mybase += wsum64[w];
       all += wsum64[w];
     }
-    if (t < n_tiles) pl.first[t] = mybase + s - count;
+    if (t < n_tiles) {
+      it.first = mybase + s - it.count;
+      pl.tiles[t] = it;
+    }
     before += all;
     __syncthreads();
   }
   if (tid == 0) *pl.n_tiles = n_tiles, *pl.total = before;
-}
-
-G4_DEV int64_t prompt_stretch(int64_t total, int wgs) {
-  const int64_t per = (total + wgs - 1) / wgs;
-  return per < PROMPT_MIN ? PROMPT_MIN : per;
+  if (before == 0) return;
+  __threadfence_block();  // the tiles, for the search
+  __syncthreads();
+  const int64_t all = before * a.kv.n_kv * pl.parts, per = prompt_stretch(all, pl.wgs);
+  for (int w = tid; w < pl.wgs; w += 1024)
+    if (w * per < all) pl.start[w] = find_tile(pl.tiles, n_tiles, w * per % before);
 }
 
 // 16 bytes a lane from src (the same in all lanes) + off to LDS at `to` + 16 * lane.
@@ -202,15 +233,6 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
   const int group = a.n_heads / kv.n_kv, units = kv.n_kv * pl.parts, n_tiles = *pl.n_tiles;
   const int64_t per_unit = *pl.total, total = per_unit * units;
 
-  // rows that see nothing
-  for (int t = blockIdx.x; t < n_tiles; t += gridDim.x)
-    if (pl.count[t] == 0) {
-      int from, to;
-      entry_rows(a, pl.entry[t], from, to);
-      const int r0 = from + pl.tok[t], r1 = min(to, r0 + pl.tt);
-      for (int64_t i = (int64_t)r0 * a.n_heads * hs + tid; i < (int64_t)r1 * a.n_heads * hs; i += 64 * NW) a.out[i] = 0.f;
-    }
-
   // Workgroups b, b + 8, ... run on one XCD: they take neighbouring stretches, so that
   // the key tiles of a kv head are read into few L2s.
   const int64_t per = prompt_stretch(total, pl.wgs);
@@ -230,31 +252,20 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
   }
   const int64_t layer_rows = (int64_t)a.layer * kv.n_pages * kv.n_kv << kv.shift;
 
-  for (int64_t u = begin; u < end;) {
-    const int hu = (int)(u / per_unit);
-    const int64_t rel = u - hu * per_unit;
-    int tile;
-    {
-      int lo = 0, hi = n_tiles - 1;  // the last tile whose first key tile is <= rel
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (pl.first[mid] <= rel) lo = mid;
-        else hi = mid - 1;
-      }
-      tile = __builtin_amdgcn_readfirstlane(lo);
-    }
-    const int cnt = __builtin_amdgcn_readfirstlane(pl.count[tile]);
-    const int j0 = __builtin_amdgcn_readfirstlane((int)(rel - pl.first[tile]));
+  if (begin >= end) return;
+  int tile = __builtin_amdgcn_readfirstlane(pl.start[stretch]), hu = (int)(begin / per_unit);
+  for (int64_t u = begin; u < end; ++tile) {
+    if (tile == n_tiles) tile = 0, ++hu;
+    const PromptTile it = pl.tiles[tile];
+    const int cnt = __builtin_amdgcn_readfirstlane(it.count);
+    if (cnt == 0) continue;
+    const int j0 = __builtin_amdgcn_readfirstlane((int)(u - hu * per_unit - it.first));
     const int j1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)cnt, j0 + (end - u)));
     const int kvh = __builtin_amdgcn_readfirstlane(hu / pl.parts);
     const int h0 = (hu - kvh * pl.parts) * pl.gh, heads = min(pl.gh, group - h0);
-    const int e = __builtin_amdgcn_readfirstlane(pl.entry[tile]), tok0 = __builtin_amdgcn_readfirstlane(pl.tok[tile]);
-    int from, to, seq;
-    entry_rows(a, e, from, to);
-    const int len = __builtin_amdgcn_readfirstlane(entry_length(a, e, seq));
-    seq = __builtin_amdgcn_readfirstlane(seq);
-    const int base = len - (to - from) + tok0;  // position of the tile's first row
-    const int toks = min(pl.tt, to - from - tok0);
+    const int seq = __builtin_amdgcn_readfirstlane(it.seq), len = __builtin_amdgcn_readfirstlane(it.len);
+    const int base = __builtin_amdgcn_readfirstlane(it.base), toks = __builtin_amdgcn_readfirstlane(it.toks);
+    const int row0 = __builtin_amdgcn_readfirstlane(it.row);
     const KeyTiles kts = key_tiles(base, base + toks - 1, a.window, a.sinks, KT);
     const int32_t *table = kv.table + (int64_t)seq * kv.max_pages;
 
@@ -268,7 +279,7 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
     const int wave_lo = base + first_tk, wave_hi = base + last_tk;
     const int wave_from0 = a.window > 0 ? max(0, max(wave_lo, 0) - a.window + 1) : 0;
     const int wave_from = a.window > 0 ? max(0, wave_hi - a.window + 1) : 0;
-    const int64_t q_row = ((int64_t)(from + tok0 + tk) * a.n_heads + kvh * group + h0 + hd) * hs;
+    const int64_t q_row = ((int64_t)(row0 + tk) * a.n_heads + kvh * group + h0 + hd) * hs;
 
     // ---- the query's parts, as B operands
     u32x4 qb[NP][STEPS];
@@ -315,18 +326,19 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
 
     // ---- loads of key tile j to a buffer: this wave's groups
     auto tile_token = [&](int j) { return (j < kts.st ? j : j - kts.st + kts.a0) * KT; };
-    auto page_at = [&](int j, int w) {  // the page of the wave's w-th group in tile j, -1 where there is none
+    // the table's entry for the wave's w-th group in tile j, read ahead (nothing looks at
+    // it until the tile's loads are issued: that would wait for the loads before it)
+    auto page_at = [&](int j, int w) {
       const int gi = (wid * IPW / IPG + w) % NT, t = tile_token(j) + gi * 16;
-      const bool in = j < j1 && t < len;
-      const int page = table[in ? t >> kv.shift : 0];
-      return in && page_ok(page, kv) ? page : -1;
+      return table[j < j1 && t < len ? t >> kv.shift : 0];
     };
     auto issue = [&](int j, int buf, const int (&pages)[UPW]) {
 #pragma unroll
       for (int w = 0; w < UPW; ++w) {
         const int unit = wid * IPW / IPG + w, gi = unit % NT, t = tile_token(j) + gi * 16;
         const bool values = unit >= NT;
-        const int page = __builtin_amdgcn_readfirstlane(pages[w]);
+        int page = __builtin_amdgcn_readfirstlane(pages[w]);
+        if (t >= len || !page_ok(page, kv)) page = -1;
         const char *src = (values ? kv.v : kv.k) +
                           uniform((layer_rows + (((int64_t)max(page, 0) * kv.n_kv + kvh) << kv.shift) + (t & (kv.page - 1))) *
                                   (int64_t)(hs * ES));
@@ -375,15 +387,23 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
 #pragma unroll
       for (int n = 0; n < NT; ++n) s[n] = f32x4{0.f, 0.f, 0.f, 0.f};
       {
+        // operands are read two products' time ahead
+        constexpr int N = STEPS * NT, AHEAD = 3;
         const int x = g4 ^ Z::k(col);
+        u32x4 k[AHEAD];
+        auto read = [&](int i) {
+          k[i % AHEAD] = *(const u32x4 *)(kt_lds + (i % NT * 16 + col) * ROW + (((4 * (i / NT)) ^ x) << 4));
+        };
 #pragma unroll
-        for (int st = 0; st < STEPS; ++st)
+        for (int i = 0; i < AHEAD - 1; ++i) read(i);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const u32x4 k = *(const u32x4 *)(kt_lds + (n * 16 + col) * ROW + (((4 * st) ^ x) << 4));
+        for (int i = 0; i < N; ++i) {
+          if (i + AHEAD - 1 < N) read(i + AHEAD - 1);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int p = NP - 1; p >= 0; --p) s[n] = M::step(k, qb[p][st], s[n]);
-          }
+          for (int p = NP - 1; p >= 0; --p) s[i % NT] = M::step(k[i % AHEAD], qb[p][i / NT], s[i % NT]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
 
       // ---- what the row sees of them
@@ -466,26 +486,37 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
         const int row = 4 * g4 + (col >> 2), vx = ((col & 3) >> 1) ^ Z::v16(row);
         const uint32_t v_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)vt_lds + row * ROW +
                               8 * (col & 1);
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4 *tr;
+        union Operand {
+          s16x4 h[2];
+          u32x4 w;
+        };
+        constexpr int N = ND * NT / 2, AHEAD = 3;
+        Operand v[AHEAD];
+        auto read = [&](int i) {
+          const uint32_t at = v_at + (((2 * (i / (NT / 2))) ^ vx) << 4) + i % (NT / 2) * 2 * GROUP;
+          v[i % AHEAD].h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr)(uintptr_t)at);
+          v[i % AHEAD].h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr)(uintptr_t)(at + GROUP));
+        };
+        f32x4 t[2];  // a sum is added while the next one is formed
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          f32x4 t = {0.f, 0.f, 0.f, 0.f};
-          const uint32_t at = v_at + (((2 * d) ^ vx) << 4);
+        for (int i = 0; i < AHEAD - 1; ++i) read(i);
 #pragma unroll
-          for (int n = 0; n < NT / 2; ++n) {
-            typedef short s16x4 __attribute__((ext_vector_type(4)));
-            typedef __attribute__((address_space(3))) s16x4 *tr;
-            union {
-              s16x4 h[2];
-              u32x4 w;
-            } v;
-            v.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr)(uintptr_t)(at + (2 * n) * GROUP));
-            v.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr)(uintptr_t)(at + (2 * n + 1) * GROUP));
+        for (int i = 0; i < N; ++i) {
+          const int d = i / (NT / 2), n = i % (NT / 2);
+          if (i + AHEAD - 1 < N) read(i + AHEAD - 1);
+          __builtin_amdgcn_sched_barrier(0);
+          if (n == 0) t[d & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int p = NP - 1; p >= 0; --p) t = M::step(v.w, pb[p][n], t);
-          }
+          for (int p = NP - 1; p >= 0; --p) t[d & 1] = M::step(v[i % AHEAD].w, pb[p][n], t[d & 1]);
+          if (n == NT / 2 - 1 && d > 0)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[d][i] = __builtin_fmaf(o[d][i], -shrunk, t[i]);
+            for (int x = 0; x < 4; ++x) o[d - 1][x] = __builtin_fmaf(o[d - 1][x], -shrunk, t[(d - 1) & 1][x]);
+          __builtin_amdgcn_sched_barrier(0);
         }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[ND - 1][x] = __builtin_fmaf(o[ND - 1][x], -shrunk, t[(ND - 1) & 1][x]);
       }
       sign = -sign;
     }
@@ -528,16 +559,15 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
   }
 }
 
-// One row from the formula, by a workgroup of four waves: LS lanes share a cached row,
+// Row `at` of the call's (row, head) pairs from the formula, by a workgroup of four waves: LS lanes share a cached row,
 // eight elements a lane, so a wave takes RS rows at a time, U of them in flight.  Each
 // group of LS lanes keeps a running maximum, sum and accumulator of the rows it has
 // met; they are joined at the end.
 template <int TYPE, int HS>
-G4_DEV void plain_row(const PagedArgs &a, int64_t out_row, int head, int seq, int pos, float *sm, float *sl, float *so) {
+G4_DEV void plain_row(const PagedArgs &a, int64_t at, int kvh, int seq, int pos, float *sm, float *sl, float *so) {
   constexpr int LS = HS / 8, RS = 64 / LS, U = 4;
   const KvArgs &kv = a.kv;
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, ql = lane % LS, rl = lane / LS;
-  const int kvh = head / (a.n_heads / kv.n_kv);
   const Seen see = seen_by(pos, a.window, a.sinks);
   const bool live = 8 * ql < kv.hs;
   const int32_t *table = kv.table + (int64_t)seq * kv.max_pages;
@@ -546,7 +576,7 @@ G4_DEV void plain_row(const PagedArgs &a, int64_t out_row, int head, int seq, in
   const float f = a.scale * LOG2E;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    q[i] = live ? a.q[(out_row * a.n_heads + head) * kv.hs + 8 * ql + i] : 0.f;
+    q[i] = live ? a.q[at * kv.hs + 8 * ql + i] : 0.f;
     acc[i] = 0.f;
   }
   for (int j0 = wid * RS * U; j0 < see.count; j0 += 4 * RS * U) {
@@ -560,9 +590,9 @@ G4_DEV void plain_row(const PagedArgs &a, int64_t out_row, int head, int seq, in
       ok[u] = page_ok(page, kv);
       kr[u].zero(), vr[u].zero();
       if (ok[u] && live) {
-        const int64_t at = (head_rows + (((int64_t)page * kv.n_kv) << kv.shift) + (t & (kv.page - 1))) * kv.hs + 8 * ql;
-        kr[u].load(kv.k, at);
-        vr[u].load(kv.v, at);
+        const int64_t row = (head_rows + (((int64_t)page * kv.n_kv) << kv.shift) + (t & (kv.page - 1))) * kv.hs + 8 * ql;
+        kr[u].load(kv.k, row);
+        vr[u].load(kv.v, row);
       }
     }
     float s[U], top = m;
@@ -608,39 +638,47 @@ G4_DEV void plain_row(const PagedArgs &a, int64_t out_row, int head, int seq, in
   __syncthreads();
   for (int d = tid; d < kv.hs; d += 256) {
     const float o = ((so[d] + so[HS + d]) + so[2 * HS + d]) + so[3 * HS + d];
-    a.out[(out_row * a.n_heads + head) * kv.hs + d] = sum == 0.f ? 0.f : o / sum;
+    a.out[at * kv.hs + d] = sum == 0.f ? 0.f : o / sum;
   }
 }
 
-// One workgroup per (query tile, kv head part): adds the slots of a tile whose key tiles
-// were spread over several stretches, in order, and computes rows again that are not finite.
+// One workgroup per (query tile, kv head part, 16 rows): adds the slots of a tile whose
+// key tiles were spread over several stretches, in order, computes rows again that are
+// not finite, and writes the zeros of rows that see nothing.
 template <int TYPE, int HS>
 __global__ __launch_bounds__(256) void k_paged_prompt_join(PagedArgs a, PromptPlan pl) {
   __shared__ float sm[4 * 8], sl[4 * 8], so[4 * HS];
-  __shared__ int32_t bad[128];
+  __shared__ int32_t bad[16];
   const KvArgs &kv = a.kv;
-  const int tid = threadIdx.x, hs = kv.hs;
+  const int tid = threadIdx.x, hs = kv.hs, words = hs / 4;
   if (*kv.status != KV_OK) return;
   const int units = kv.n_kv * pl.parts, tile = blockIdx.x / units, hu = blockIdx.x - tile * units;
   if (tile >= *pl.n_tiles) return;
-  const int cnt = pl.count[tile];
-  if (cnt == 0) return;
+  const PromptTile it = pl.tiles[tile];
   const int64_t per_unit = *pl.total, per = prompt_stretch(per_unit * units, pl.wgs);
-  const int64_t ua = hu * per_unit + pl.first[tile];
-  const int w0 = (int)(ua / per), w1 = (int)((ua + cnt - 1) / per);
   const int group = a.n_heads / kv.n_kv, kvh = hu / pl.parts, h0 = (hu - kvh * pl.parts) * pl.gh;
-  const int heads = min(pl.gh, group - h0), e = pl.entry[tile], tok0 = pl.tok[tile];
-  int from, to, seq;
-  entry_rows(a, e, from, to);
-  const int len = entry_length(a, e, seq), rows = min(pl.tt, to - from - tok0) * heads;
-  if (tid < 128) bad[tid] = 0;
+  const int heads = min(pl.gh, group - h0), r0 = blockIdx.y * 16, r1 = min(r0 + 16, it.toks * heads);
+  if (r0 >= r1) return;
+  auto out_at = [&](int r, int &tk) {  // the call's (row, head) of the tile's row r
+    tk = r / heads;
+    return (int64_t)(it.row + tk) * a.n_heads + kvh * group + h0 + (r - tk * heads);
+  };
+  int tk;
+  if (it.count == 0) {
+    for (int i = tid; i < (r1 - r0) * words; i += 256)
+      *(float4 *)(a.out + out_at(r0 + i / words, tk) * hs + 4 * (i % words)) = make_float4(0, 0, 0, 0);
+    return;
+  }
+  const int64_t ua = hu * per_unit + it.first;
+  const int w0 = (int)(ua / per), w1 = (int)((ua + it.count - 1) / per);
+  if (tid < 16) bad[tid] = 0;
   __syncthreads();
   if (w0 != w1) {
     const int64_t s0 = 2 * (int64_t)w0 + (ua != w0 * per);
-    const int words = hs / 4;
-    for (int i = tid; i < rows * words; i += 256) {
-      const int r = i / words, x = i - r * words;
+    for (int i = tid; i < (r1 - r0) * words; i += 256) {
+      const int r = r0 + i / words, x = i % words;
       float top = -__builtin_inff();
+#pragma unroll 4
       for (int w = w0; w <= w1; ++w) top = fmaxf(top, pl.ml[((w == w0 ? s0 : 2 * (int64_t)w) * pl.bm + r) * 2]);
       float4 o = make_float4(0, 0, 0, 0);
       float sum = 0.f;
@@ -655,20 +693,19 @@ __global__ __launch_bounds__(256) void k_paged_prompt_join(PagedArgs a, PromptPl
       }
       const bool none = sum == 0.f;
       o.x = none ? 0.f : o.x / sum, o.y = none ? 0.f : o.y / sum, o.z = none ? 0.f : o.z / sum, o.w = none ? 0.f : o.w / sum;
-      const int tk = r / heads, hd = r - tk * heads;
-      *(float4 *)(a.out + ((int64_t)(from + tok0 + tk) * a.n_heads + kvh * group + h0 + hd) * hs + 4 * x) = o;
+      *(float4 *)(a.out + out_at(r, tk) * hs + 4 * x) = o;
       if (!(__builtin_fabsf(o.x) < __builtin_inff()) || !(__builtin_fabsf(o.y) < __builtin_inff()) ||
           !(__builtin_fabsf(o.z) < __builtin_inff()) || !(__builtin_fabsf(o.w) < __builtin_inff()))
-        bad[r] = 1;
+        bad[r - r0] = 1;
     }
-  } else if (tid < rows) {
-    bad[tid] = pl.odd[(int64_t)blockIdx.x * (pl.bm / 16) + (tid >> 4)] >> (tid & 15) & 1;
+  } else if (tid < r1 - r0) {
+    bad[tid] = pl.odd[(int64_t)blockIdx.x * (pl.bm / 16) + blockIdx.y] >> tid & 1;
   }
-  if (!__syncthreads_or(tid < 128 && bad[tid])) return;
-  for (int r = 0; r < rows; ++r) {
-    if (!bad[r]) continue;
-    const int tk = r / heads, hd = r - tk * heads;
-    plain_row<TYPE, HS>(a, from + tok0 + tk, kvh * group + h0 + hd, seq, len - (to - from) + tok0 + tk, sm, sl, so);
+  __syncthreads();
+  for (int r = r0; r < r1; ++r) {
+    if (!bad[r - r0]) continue;
+    const int64_t at = out_at(r, tk);
+    plain_row<TYPE, HS>(a, at, kvh, it.seq, it.base + tk, sm, sl, so);
   }
 }
 
@@ -692,10 +729,8 @@ static size_t prompt_layout(const PagedArgs &a, const DevInfo &dev, char *base, 
   const size_t cap = (size_t)p->cap, units = (size_t)a.kv.n_kv * p->parts;
   p->n_tiles = (int32_t *)add(4);
   p->total = (int64_t *)add(8);
-  p->first = (int64_t *)add(8 * cap);
-  p->count = (int32_t *)add(4 * cap);
-  p->entry = (int32_t *)add(4 * cap);
-  p->tok = (int32_t *)add(4 * cap);
+  p->start = (int32_t *)add(4 * (size_t)p->wgs);
+  p->tiles = (PromptTile *)add(sizeof(PromptTile) * cap);
   p->odd = (uint16_t *)add(2 * cap * units * (p->bm / 16));
   p->part = (float *)add(sizeof(float) * 2 * (size_t)p->wgs * p->bm * a.kv.hs);
   p->ml = (float *)add(sizeof(float) * 4 * (size_t)p->wgs * p->bm);
@@ -713,7 +748,8 @@ static hipError_t launch_tiles(const PagedArgs &a, const PromptPlan &p, hipStrea
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   constexpr int JHS = HS == 96 ? 128 : HS == 192 ? 256 : HS;
-  hipLaunchKernelGGL((k_paged_prompt_join<TYPE, JHS>), dim3(p.cap * a.kv.n_kv * p.parts), dim3(256), 0, s, a, p);
+  hipLaunchKernelGGL((k_paged_prompt_join<TYPE, JHS>), dim3(p.cap * a.kv.n_kv * p.parts, p.bm / 16), dim3(256), 0, s,
+                     a, p);
   return hipGetLastError();
 }
 
