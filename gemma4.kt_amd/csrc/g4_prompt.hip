@@ -191,6 +191,9 @@ G4_DEV void load_to_lds(const char *src, uint32_t off, uint32_t to) {
 // The loads to LDS and the LDS operations of the wave are done; then all waves meet.
 G4_DEV void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// Operands read ahead of the product that takes them.
+constexpr int prompt_ahead(int type, int hs) { return type == T_BF16 ? 4 : 6; }
+
 constexpr int prompt_waves(int hs) { return hs > 256 ? 4 : 8; }
 constexpr int prompt_kt(int type, int hs) {
   const int es = type == T_F32 ? 4 : 2, kt = 32768 / (hs * es);
@@ -220,9 +223,8 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
   constexpr int NP = TYPE == T_BF16 ? 3 : TYPE == T_F16 ? 2 : 1;  // parts of a query or weight
   constexpr int STEPS = HS / M::STEP, NT = KT / 16, ND = HS / 16;
   constexpr int CH = HS * ES / 16, ROW = HS * ES, GROUP = 16 * ROW, HALF = KT * ROW;
-  constexpr int IPW = 2 * KT * CH / 64 / NW, IPG = CH / 4;  // 1 KB loads of a wave, of a 16-token group
-  static_assert(IPW >= 1 && IPW * NW * 64 == 2 * KT * CH && (IPG % IPW == 0 || IPW % IPG == 0), "loads of a tile");
-  constexpr int UPW = IPW > IPG ? IPW / IPG : 1, IPU = IPW / UPW;  // groups (of keys or values) a wave loads, loads of each
+  constexpr int GW = 4 / NT, IPW = CH / 4 / GW;  // waves that load a 16-token group, 1 KB loads of each
+  static_assert(NT * GW == 4 && IPW * GW * 64 == 16 * CH, "loads of a tile");
   using Z = Swz<CH>;
   __shared__ __align__(1024) char lds[4 * HALF];  // [buffer][keys, values][KT][ROW]
   __shared__ int32_t okf[2][NT];                  // the groups' pages are there
@@ -242,14 +244,6 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
   const int col = lane & 15, g4 = lane >> 4;  // row of the tile's 16; quarter of a step, or of a key tile's 16
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
 
-  // ---- where this lane's 16 bytes of each load come from, within a group's rows of a head
-  uint32_t src_off[IPW];
-#pragma unroll
-  for (int i = 0; i < IPW; ++i) {
-    const int unit = (wid * IPW + i) / IPG, at = (wid * IPW + i) % IPG * 64 + lane;
-    const int row = at / CH, c = at % CH, swz = unit < NT ? Z::k(row) : F32 ? Z::v32(row) : Z::v16(row);
-    src_off[i] = (uint32_t)(row * hs * ES + min((c ^ swz) * 16, hs * ES - 16));
-  }
   const int64_t layer_rows = (int64_t)a.layer * kv.n_pages * kv.n_kv << kv.shift;
 
   if (begin >= end) return;
@@ -324,111 +318,137 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
     float m = -__builtin_inff(), l = 0.f;
     float sign = 1.f;
 
-    // ---- loads of key tile j to a buffer: this wave's groups
+    // ---- loads of key tiles, by the last four waves: each a group's keys and values, or
+    // a part of them
+    const int loader = wid - (NW - 4), gi = loader / GW, part = loader % GW;
     auto tile_token = [&](int j) { return (j < kts.st ? j : j - kts.st + kts.a0) * KT; };
-    // the table's entry for the wave's w-th group in tile j, read ahead (nothing looks at
-    // it until the tile's loads are issued: that would wait for the loads before it)
-    auto page_at = [&](int j, int w) {
-      const int gi = (wid * IPW / IPG + w) % NT, t = tile_token(j) + gi * 16;
+    // the table's entry for the wave's group in tile j, read ahead (nothing looks at it
+    // until the tile's loads are issued: that would wait for the loads before it)
+    auto page_at = [&](int j) {
+      const int t = tile_token(j) + gi * 16;
       return table[j < j1 && t < len ? t >> kv.shift : 0];
     };
-    auto issue = [&](int j, int buf, const int (&pages)[UPW]) {
+    int next_page = 0;
+    auto issue = [&](int j) {
+      const int t = tile_token(j) + gi * 16, buf = (j - j0) & 1;
+      int page = __builtin_amdgcn_readfirstlane(next_page);
+      if (t >= len || !page_ok(page, kv)) page = -1;
+      const int64_t row0 = uniform(
+          (layer_rows + (((int64_t)max(page, 0) * kv.n_kv + kvh) << kv.shift) + (t & (kv.page - 1))) * (int64_t)(hs * ES));
+      const uint32_t to = buf * 2 * HALF + gi * GROUP + part * IPW * 1024;
+      if (part == 0 && lane == 0) okf[buf][gi] = page >= 0;
+      // The lane's 16 bytes of load i: word c of a row of the group.  Formed for each tile:
+      // kept over the loop these places would take the registers of the sums.
+      const int ln = (int)opaque((uint32_t)lane);
+      auto from = [&](int i, bool values) {
+        const int at = (part * IPW + i) * 64 + ln, row = at / CH, c = at % CH;
+        const int swz = !values ? Z::k(row) : F32 ? Z::v32(row) : Z::v16(row);
+        return (uint32_t)(row * hs * ES + min((c ^ swz) * 16, hs * ES - 16));
+      };
+      // Whole rows of a power of two of words: the loads differ from the first one by their
+      // rows and a change of the word's low bits.
+      constexpr bool POW2 = (CH & (CH - 1)) == 0 && CH <= 64;
+      const bool fast = POW2 && hs == HS;
+      auto load = [&](const char *src, uint32_t first, uint32_t at, int i, bool values) {
+        constexpr int R = 64 / CH > 0 ? 64 / CH : 1;  // rows of a load
+        const int row = (part * IPW + i) * R;  // the same in all lanes
+        const int swz = !values ? Z::k(row) : F32 ? Z::v32(row) : Z::v16(row);
+        load_to_lds(src + row * ROW, first ^ (uint32_t)(swz << 4), at + i * 1024);
+      };
+      const int lrow = ln / CH, lc = ln % CH;
+      if (page >= 0 && fast) {
+        const uint32_t first = lrow * ROW + ((lc ^ Z::k(lrow)) << 4);
 #pragma unroll
-      for (int w = 0; w < UPW; ++w) {
-        const int unit = wid * IPW / IPG + w, gi = unit % NT, t = tile_token(j) + gi * 16;
-        const bool values = unit >= NT;
-        int page = __builtin_amdgcn_readfirstlane(pages[w]);
-        if (t >= len || !page_ok(page, kv)) page = -1;
-        const char *src = (values ? kv.v : kv.k) +
-                          uniform((layer_rows + (((int64_t)max(page, 0) * kv.n_kv + kvh) << kv.shift) + (t & (kv.page - 1))) *
-                                  (int64_t)(hs * ES));
-        const int first = wid * IPW % IPG;  // load of the group this wave begins with
-        const uint32_t to_off = buf * 2 * HALF + (values ? HALF : 0) + gi * GROUP + first * 1024;
-        if (!values && first == 0 && lane == 0) okf[buf][gi] = page >= 0;
-        if (values && (page < 0 || t + 16 > len)) {
-          // rows that hold no token: zeros, since a weight of zero does not silence a NaN
+        for (int i = 0; i < IPW; ++i) load(kv.k + row0, first, lds0 + to, i, false);
+      } else if (page >= 0) {
 #pragma unroll
-          for (int i = 0; i < IPU; ++i) {
-            const int row = ((first + i) * 64 + lane) / CH;
-            u32x4 v = *(const u32x4 *)(src + src_off[w * IPU + i]);
-            const bool in = page >= 0 && t + row < len;
+        for (int i = 0; i < IPW; ++i) load_to_lds(kv.k + row0, from(i, false), lds0 + to + i * 1024);
+      }
+      if (page >= 0 && t + 16 <= len) {
+        if (fast) {
+          const uint32_t first = lrow * ROW + ((lc ^ (F32 ? Z::v32(lrow) : Z::v16(lrow))) << 4);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) v[x] = in ? v[x] : 0u;
-            *(u32x4 *)(lds + to_off + i * 1024 + lane * 16) = v;
-          }
-        } else if (page >= 0) {
+          for (int i = 0; i < IPW; ++i) load(kv.v + row0, first, lds0 + HALF + to, i, true);
+        } else {
 #pragma unroll
-          for (int i = 0; i < IPU; ++i) load_to_lds(src, src_off[w * IPU + i], lds0 + to_off + i * 1024);
+          for (int i = 0; i < IPW; ++i) load_to_lds(kv.v + row0, from(i, true), lds0 + HALF + to + i * 1024);
         }
+      } else {
+        // rows that hold no token: zeros, since a weight of zero does not silence a NaN
+#pragma unroll
+        for (int i = 0; i < IPW; ++i) {
+          const int row = ((part * IPW + i) * 64 + ln) / CH;
+          u32x4 v = *(const u32x4 *)(kv.v + row0 + from(i, true));
+          const bool in = page >= 0 && t + row < len;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) v[x] = in ? v[x] : 0u;
+          *(u32x4 *)(lds + HALF + to + i * 1024 + lane * 16) = v;
+        }
+      }
+      next_page = page_at(j + 1);
+    };
+
+    f32x4 s[NT];                                     // scores: s[n][i] of key 16 n + 4 g4 + i, then weights
+    u32x4 pb[F32 ? 1 : NP][F32 ? 1 : (NT + 1) / 2];  // the weights' parts
+    float shrunk = 0.f;                              // what the sums so far shrink by
+    uint32_t there = 0;                              // groups of the scored tile whose pages are there
+    bool scored = false, weighted = false;           // s holds a tile's scores; its weights wait for the values
+
+    auto score = [&](int j) {
+      const int t0 = tile_token(j), buf = (j - j0) & 1;
+      scored = wave_on && t0 <= wave_hi && (t0 + KT > wave_from0 || t0 < a.sinks);  // else nothing is seen
+      if (!scored) return;
+      there = 0;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) there |= (uint32_t)__builtin_amdgcn_readfirstlane(okf[buf][n]) << n;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+      // the steps' places in a row: four patterns of its low bits.  They are formed ahead,
+      // since an address formed between products waits for the one that had its register.
+      typedef __attribute__((address_space(3))) const u32x4 *words;
+      uint32_t pat[4];
+      const int at_col = (int)opaque((uint32_t)col);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        pat[i] = lds0 + buf * 2 * HALF + at_col * ROW + (((4 * i) ^ g4 ^ Z::k(at_col)) << 4);
+        asm volatile("" : "+v"(pat[i]));
+      }
+      constexpr int N = STEPS * NT, A = prompt_ahead(TYPE, HS);
+      u32x4 k[A + 1];
+      auto read = [&](int i) {
+        const int st = i / NT;
+        k[i % (A + 1)] = *(words)(uintptr_t)(pat[st & 3] + (i % NT * 16 * ROW + (st >> 2) * 256));
+      };
+#pragma unroll
+      for (int i = 0; i < A; ++i) read(i);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (i + A < N) read(i + A);
+#pragma unroll
+        for (int p = NP - 1; p >= 0; --p) s[i % NT] = M::step(k[i % (A + 1)], qb[p][i / NT], s[i % NT]);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // the read behind the first product
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_barrier(0);
       }
     };
 
-    int pages[UPW];
-#pragma unroll
-    for (int w = 0; w < UPW; ++w) pages[w] = page_at(j0, w);
-    tile_barrier();  // the last segment's tiles are done with
-    issue(j0, 0, pages);
-#pragma unroll
-    for (int w = 0; w < UPW; ++w) pages[w] = page_at(j0 + 1, w);
-
-    for (int j = j0; j < j1; ++j) {
-      const int buf = (j - j0) & 1, t0 = tile_token(j);
-      tile_barrier();  // tile j is here, and everyone is done with tile j - 1
-      if (j + 1 < j1) {
-        issue(j + 1, buf ^ 1, pages);
-#pragma unroll
-        for (int w = 0; w < UPW; ++w) pages[w] = page_at(j + 2, w);
-      }
-      if (!wave_on || t0 > wave_hi || (t0 + KT <= wave_from0 && t0 >= a.sinks)) continue;  // nothing seen
-      const char *kt_lds = lds + buf * 2 * HALF, *vt_lds = kt_lds + HALF;
-
-      // ---- scores of the tile: s[n][i] of key 16 n + 4 g4 + i
-      f32x4 s[NT];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) s[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-      {
-        // operands are read two products' time ahead
-        constexpr int N = STEPS * NT, AHEAD = 3;
-        const int x = g4 ^ Z::k(col);
-        u32x4 k[AHEAD];
-        auto read = [&](int i) {
-          k[i % AHEAD] = *(const u32x4 *)(kt_lds + (i % NT * 16 + col) * ROW + (((4 * (i / NT)) ^ x) << 4));
-        };
-#pragma unroll
-        for (int i = 0; i < AHEAD - 1; ++i) read(i);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          if (i + AHEAD - 1 < N) read(i + AHEAD - 1);
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int p = NP - 1; p >= 0; --p) s[i % NT] = M::step(k[i % AHEAD], qb[p][i / NT], s[i % NT]);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      }
-
-      // ---- what the row sees of them
-      bool all_pages = true;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) all_pages &= __builtin_amdgcn_readfirstlane(okf[buf][n]) != 0;
-      const bool full = all_pages && t0 + KT - 1 <= wave_lo && (t0 >= wave_from || t0 + KT - 1 < a.sinks);
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[n][i] *= back;
+    auto weigh = [&](int j) {
+      weighted = scored;
+      if (!scored) return;
+      scored = false;
+      const int t0 = tile_token(j);
+      const bool full = there == (1u << NT) - 1 && t0 + KT - 1 <= wave_lo && (t0 >= wave_from || t0 + KT - 1 < a.sinks);
       if (!full) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const bool there = okf[buf][n] != 0;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int t = t0 + n * 16 + 4 * g4 + i;
-            const bool seen = there && t <= pos && (t >= seen_from || t < a.sinks);
+            const bool seen = (there >> n & 1) && t <= pos && (t >= seen_from || t < a.sinks);
             s[n][i] = seen ? s[n][i] : -__builtin_inff();
           }
-        }
       }
-
-      // ---- weights
       float top = s[0][0];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -436,25 +456,53 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
         for (int i = 0; i < 4; ++i) top = fmaxf(top, s[n][i]);
       top = fmaxf(top, __uint_as_float(partner_u32<16>(__float_as_uint(top), lane)));
       top = fmaxf(top, __uint_as_float(partner_u32<32>(__float_as_uint(top), lane)));
-      top = fmaxf(m, top);
+      top = fmaxf(m, top * back);
       // weights of F16 stand 2^14 higher, so that the second part of a small one is not subnormal
       const float up = TYPE == T_F16 ? 14.f : 0.f;
       const float zero = top == -__builtin_inff() ? 0.f : top - up;
-      const float shrunk = __builtin_amdgcn_exp2f(m - (zero + up));
+      shrunk = __builtin_amdgcn_exp2f(m - (zero + up));
       m = top;
       float sum = 0.f;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float w = __builtin_amdgcn_exp2f(s[n][i] - zero);
+          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], back, -zero));  // the product is exact
           sum += w;
-          s[n][i] = w * sign;
+          s[n][i] = F32 ? w * sign : w;
         }
       l = __builtin_fmaf(l, shrunk, sum);
+      if constexpr (!F32) {
+        const uint32_t flip = sign < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+        for (int n = 0; n < NT / 2; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = 2 * n + (i >> 1), x = 2 * (i & 1);
+            float w0 = s[k][x], w1 = s[k][x + 1];
+            if constexpr (TYPE == T_F16) {
+              // the first part truncated, the remainder exact, the second to nearest
+              const auto hi = __builtin_amdgcn_cvt_pkrtz(w0, w1);
+              typedef float f32x2 __attribute__((ext_vector_type(2)));
+              typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+              const f16x2 lo = __builtin_convertvector((f32x2{w0 - (float)hi[0], w1 - (float)hi[1]}), f16x2);
+              pb[0][n][i] = __builtin_bit_cast(uint32_t, hi) ^ flip;
+              pb[1][n][i] = __builtin_bit_cast(uint32_t, lo) ^ flip;
+            } else {
+#pragma unroll
+              for (int p = 0; p < NP; ++p) pb[p][n][i] = take_part<TYPE>(w0, w1) ^ flip;
+            }
+          }
+      }
+    };
 
-      // ---- O^T = shrunk O^T + V^T P^T
+    // O^T = shrunk O^T + V^T P^T, o holding the sums times the last tile's sign
+    auto add_values = [&](int j) {
+      if (!weighted) return;
+      weighted = false;
+      const int buf = (j - j0) & 1;
       if constexpr (F32) {
+        const char *vt_lds = lds + buf * 2 * HALF + HALF;
         const int vx = Z::v32(4 * g4);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
@@ -471,54 +519,67 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
           for (int i = 0; i < 4; ++i) o[d][i] = __builtin_fmaf(o[d][i], -shrunk, t[i]);
         }
       } else {
-        u32x4 pb[NP][NT / 2];
-#pragma unroll
-        for (int n = 0; n < NT / 2; ++n)
-#pragma unroll
-          for (int p = 0; p < NP; ++p)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int k = 2 * n + (i >> 1), x = 2 * (i & 1);
-              float w0 = s[k][x], w1 = s[k][x + 1];
-              pb[p][n][i] = take_part<TYPE>(w0, w1);
-              s[k][x] = w0, s[k][x + 1] = w1;
-            }
-        const int row = 4 * g4 + (col >> 2), vx = ((col & 3) >> 1) ^ Z::v16(row);
-        const uint32_t v_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)vt_lds + row * ROW +
-                              8 * (col & 1);
+        const int at_col = (int)opaque((uint32_t)col), row = 4 * g4 + (at_col >> 2), vx = ((at_col & 3) >> 1) ^ Z::v16(row);
+        const uint32_t v_at = lds0 + buf * 2 * HALF + HALF + row * ROW + 8 * (at_col & 1);
         typedef short s16x4 __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) s16x4 *tr;
         union Operand {
           s16x4 h[2];
           u32x4 w;
         };
-        constexpr int N = ND * NT / 2, AHEAD = 3;
-        Operand v[AHEAD];
+        // 16 elements of the head after the other, over 32 keys a product
+        constexpr int N = ND * NT / 2, A = prompt_ahead(TYPE, HS);
+        Operand v[A + 1];
+        uint32_t pat[8];  // as for the keys
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          pat[i] = v_at + (((2 * i) ^ vx) << 4);
+          asm volatile("" : "+v"(pat[i]));
+        }
         auto read = [&](int i) {
-          const uint32_t at = v_at + (((2 * (i / (NT / 2))) ^ vx) << 4) + i % (NT / 2) * 2 * GROUP;
-          v[i % AHEAD].h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr)(uintptr_t)at);
-          v[i % AHEAD].h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr)(uintptr_t)(at + GROUP));
+          const int d = i / (NT / 2), n = i % (NT / 2);
+          const uint32_t at = pat[d & 7] + (d >> 3) * 256 + n * 2 * GROUP;
+          v[i % (A + 1)].h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr)(uintptr_t)at);
+          v[i % (A + 1)].h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr)(uintptr_t)(at + GROUP));
         };
         f32x4 t[2];  // a sum is added while the next one is formed
 #pragma unroll
-        for (int i = 0; i < AHEAD - 1; ++i) read(i);
+        for (int i = 0; i < A; ++i) read(i);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const int d = i / (NT / 2), n = i % (NT / 2);
-          if (i + AHEAD - 1 < N) read(i + AHEAD - 1);
-          __builtin_amdgcn_sched_barrier(0);
+          if (i + A < N) read(i + A);
           if (n == 0) t[d & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int p = NP - 1; p >= 0; --p) t[d & 1] = M::step(v[i % AHEAD].w, pb[p][n], t[d & 1]);
+          for (int p = NP - 1; p >= 0; --p) t[d & 1] = M::step(v[i % (A + 1)].w, pb[p][n], t[d & 1]);
           if (n == NT / 2 - 1 && d > 0)
 #pragma unroll
             for (int x = 0; x < 4; ++x) o[d - 1][x] = __builtin_fmaf(o[d - 1][x], -shrunk, t[(d - 1) & 1][x]);
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
           __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int x = 0; x < 4; ++x) o[ND - 1][x] = __builtin_fmaf(o[ND - 1][x], -shrunk, t[(ND - 1) & 1][x]);
       }
       sign = -sign;
+    };
+
+    // The loads of a tile's successor take their waves a while to issue.  The other wave
+    // of each of their SIMDs begins with the tile at once and so stays ahead: one has the
+    // matrix cores while the other forms weights.
+    if (loader >= 0) next_page = page_at(j0);
+    tile_barrier();  // the last segment's tiles are done with
+    if (loader >= 0) issue(j0);
+    for (int j = j0; j < j1; ++j) {
+      tile_barrier();  // tile j is here, and everyone is done with tile j - 1
+      if (loader >= 0 && j + 1 < j1) issue(j + 1);
+      score(j);
+      weigh(j);
+      add_values(j);
     }
 
     // ---- the segment's result
