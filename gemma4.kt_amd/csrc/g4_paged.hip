@@ -29,8 +29,6 @@ namespace g4 {
 // elements of a row per lane, with the weights handed over through the wave's own LDS.
 // While a tile is worked on, the next one's keys and values are on their way.
 
-constexpr int SPLIT_MIN = 8;  // least groups of a stretch
-
 // A row's visible tokens as groups: the first gs, then those from g0.
 struct Groups {
   int count;
@@ -69,9 +67,17 @@ struct SplitPlan {
   int32_t gt;
 };
 
-G4_DEV int64_t stretch_of(int64_t total, int wgs) {
-  const int64_t per = (total + wgs - 1) / wgs;
-  return per < SPLIT_MIN ? SPLIT_MIN : per;
+// a / b for a >= 0, b > 0; long division only where the numbers are long
+G4_DEV int64_t quotient(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
+// Units of a stretch: an equal share, but at least a group for each of a workgroup's four
+// waves, where heads have that many.
+G4_DEV int64_t stretch_of(int64_t total, int wgs, int heads) {
+  const int64_t per = quotient(total + wgs - 1, wgs), mean = quotient(total + heads - 1, heads);
+  const int64_t least = mean < 1 ? 1 : mean > 4 ? 4 : mean;
+  return per < least ? least : per;
 }
 
 // A score whose products or sums the matrix cores could not form (an infinite key times
@@ -90,7 +96,7 @@ G4_DEV float plain_score(const float *q, const char *k, int hs, float f) {
   return d * f;
 }
 
-template <int TYPE, int HS, int GT>
+template <int TYPE, int HS, int GT, bool FULL>
 __global__ __launch_bounds__(256, split_per_cu(TYPE, HS, GT)) void k_paged_split(PagedArgs a, SplitPlan pl) {
   using M = Mfma<TYPE>;
   constexpr int ES = TYPE == T_F32 ? 4 : 2, RW = TYPE == T_F32 ? 2 : 1;
@@ -100,17 +106,17 @@ __global__ __launch_bounds__(256, split_per_cu(TYPE, HS, GT)) void k_paged_split
   constexpr int QOP = SETS * STEPS * 64 * 16, SO = 4 * GT * HS * 4;
   __shared__ __align__(16) char shared[QOP > SO ? QOP : SO];
   __shared__ float pw[4][NG * 16][GT];
-  __shared__ float sm[4][GT], sl[4][GT], back[SETS * 4];
+  __shared__ float sm[4][GT], sl[4][GT], stat[GT][2], back[SETS * 4];
   __shared__ int64_t wsum[4];
-  extern __shared__ __align__(16) char dyn[];  // first [n + 1], count [n], length [n]
+  extern __shared__ __align__(16) char dyn[];  // first [n + 1], count [n], length [n], sequence [n]
   u32x4(*qop)[64] = (u32x4(*)[64])shared;
   float(*so)[GT][HS] = (float(*)[GT][HS])shared;
   int64_t *first = (int64_t *)dyn;
-  int32_t *count = (int32_t *)(first + a.n + 1), *length = count + a.n;
+  int32_t *count = (int32_t *)(first + a.n + 1), *length = count + a.n, *sequence = length + a.n;
 
   const KvArgs &kv = a.kv;
-  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), hs = kv.hs;
-  if (*kv.status != KV_OK) return;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), hs = FULL ? HS : kv.hs;
+  const int status = *kv.status;  // looked at once the lengths are here too
   const int group = a.n_heads / kv.n_kv, units = kv.n_kv * pl.parts;
 
   // ---- the units before each row: four rows a thread
@@ -128,6 +134,7 @@ __global__ __launch_bounds__(256, split_per_cu(TYPE, HS, GT)) void k_paged_split
         c[j] = groups_of(len - 1, a.window, a.sinks).count;
         count[e] = c[j];
         length[e] = len;
+        sequence[e] = (unsigned)seq < (unsigned)kv.max_seqs ? seq : 0;
         mine += (int64_t)c[j] * units;
       }
     }
@@ -150,6 +157,7 @@ __global__ __launch_bounds__(256, split_per_cu(TYPE, HS, GT)) void k_paged_split
     }
     __syncthreads();
   }
+  if (status != KV_OK) return;
   if (blockIdx.x == 0) {
     for (int e = tid; e <= a.n; e += 256) {
       pl.first[e] = first[e];
@@ -160,7 +168,7 @@ __global__ __launch_bounds__(256, split_per_cu(TYPE, HS, GT)) void k_paged_split
     if (count[e] == 0)
       for (int i = tid; i < a.n_heads * hs; i += 256) a.out[(int64_t)e * a.n_heads * hs + i] = 0.f;
 
-  const int64_t per = stretch_of(first[a.n], gridDim.x);
+  const int64_t per = stretch_of(first[a.n], gridDim.x, a.n * units);
   const int64_t begin = blockIdx.x * per, end = min(first[a.n], begin + per);
   const float f = a.scale * LOG2E;
   const int key = lane & 15, kq = lane >> 4;  // of a score; of a key's dims
@@ -179,71 +187,14 @@ __global__ __launch_bounds__(256, split_per_cu(TYPE, HS, GT)) void k_paged_split
     }
     const int cnt = count[e];
     const int64_t rel = u - first[e];
-    const int hu = __builtin_amdgcn_readfirstlane((int)(rel / cnt));
+    const int hu = __builtin_amdgcn_readfirstlane((int)quotient(rel, cnt));
     const int gi0 = __builtin_amdgcn_readfirstlane((int)(rel - (int64_t)hu * cnt));
     const int gi1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)cnt, gi0 + (end - u)));
     const int kvh = hu / pl.parts, h0 = (hu - kvh * pl.parts) * GT, heads = min(GT, group - h0);
-    const int seq = __builtin_amdgcn_readfirstlane(a.seqs[e]);
+    const int seq = __builtin_amdgcn_readfirstlane(sequence[e]);
     const int pos = __builtin_amdgcn_readfirstlane(length[e]) - 1;
     const Groups g = groups_of(pos, a.window, a.sinks);
     const float *q0 = a.q + ((int64_t)e * a.n_heads + kvh * group + h0) * hs;
-
-    // ---- the queries as A operands: wave w takes heads w and w + 4, lane c dims 8c .. 8c + 7
-    __syncthreads();
-#pragma unroll
-    for (int h = wid; h < SETS * 4; h += 4) {
-      float x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = 0.f;
-      if (h < heads && 8 * lane < hs) {
-        const float4 y = ((const float4 *)(q0 + (int64_t)h * hs))[2 * lane];
-        const float4 z = ((const float4 *)(q0 + (int64_t)h * hs))[2 * lane + 1];
-        x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w, x[4] = z.x, x[5] = z.y, x[6] = z.z, x[7] = z.w;
-      }
-      float top = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] *= f;
-        top = fmaxf(top, __builtin_fabsf(x[i]));
-      }
-      top = lanes16_max(top, lane);
-      top = fmaxf(top, __uint_as_float(partner_u32<16>(__float_as_uint(top), lane)));
-      top = fmaxf(top, __uint_as_float(partner_u32<32>(__float_as_uint(top), lane)));
-      float to, bk;
-      split_scale<TYPE>(top, to, bk);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] *= to;
-      if (lane == 0) back[h] = bk;
-      if (8 * lane < HS) {
-        const int row = 4 * (h & 3);
-        if constexpr (TYPE == T_F32) {
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int d = 8 * lane + 4 * half, at = (h >> 2) * STEPS + d / 16, l0 = (d % 16) / 4 * 16 + row;
-            u32x4 w;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(x[4 * half + i]);
-            qop[at][l0] = w;
-#pragma unroll
-            for (int r = 1; r < 4; ++r) qop[at][l0 + r] = u32x4{0, 0, 0, 0};
-          }
-        } else {
-          const int at = (h >> 2) * STEPS + lane / 4, l0 = (lane & 3) * 16 + row;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            u32x4 w = {0, 0, 0, 0};
-            if (r < 3)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) w[i] = take_part<TYPE>(x[2 * i], x[2 * i + 1]);
-            qop[at][l0 + r] = w;
-          }
-        }
-      }
-    }
-    __syncthreads();
-    float bk[SETS];
-#pragma unroll
-    for (int s = 0; s < SETS; ++s) bk[s] = back[s * 4 + kq];
 
     // ---- this wave's groups
     const int share = (gi1 - gi0 + 3) >> 2;
@@ -259,6 +210,20 @@ __global__ __launch_bounds__(256, split_per_cu(TYPE, HS, GT)) void k_paged_split
       const int page = __builtin_amdgcn_readlane(pids, i);
       return page_ok(page, kv) ? page : -1;
     };
+    const int pids0 = load_pages(wa);
+
+    // ---- the queries: wave w takes heads w and w + 4, lane c dims 8c .. 8c + 7
+    float x[SETS][8];
+#pragma unroll
+    for (int s = 0; s < SETS; ++s) {
+      const bool in = 4 * s + wid < heads && 8 * lane < hs;
+      const float4 *at = (const float4 *)(q0 + (in ? (int64_t)(4 * s + wid) * hs + 8 * lane : 0));
+      const float4 y = at[0], z = at[1];
+      x[s][0] = y.x, x[s][1] = y.y, x[s][2] = y.z, x[s][3] = y.w, x[s][4] = z.x, x[s][5] = z.y, x[s][6] = z.z, x[s][7] = z.w;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[s][i] = in ? x[s][i] : 0.f;
+    }
+
     float acc[GT][8], m[SETS], l[SETS];
 #pragma unroll
     for (int h = 0; h < GT; ++h)
@@ -275,23 +240,30 @@ __global__ __launch_bounds__(256, split_per_cu(TYPE, HS, GT)) void k_paged_split
     };
     // Lanes whose elements lie behind the head read its last ones again: the query is zero
     // there, and what they make of the values is not used.
+    // Buffer loads: a group's rows of the head from a scalar base, 32 bits of offset a lane,
+    // bounded by the hardware.
     const int kd = kq * (M::STEP / 4), k_last = hs - M::STEP / 4;
-    const uint32_t k_row = (uint32_t)(key * hs * ES), v_off = (uint32_t)(rl * hs + min(8 * ql, hs - 8)) * ES;
+    const uint32_t k_off = (uint32_t)(key * hs + (FULL ? kd : 0)) * ES;
+    const uint32_t v_off = (uint32_t)(rl * hs + min(8 * ql, hs - 8)) * ES;
     auto load_k = [&](int n, int64_t row) {
-      const char *at = kv.k + uniform(row);
+      const auto at = __builtin_amdgcn_make_buffer_rsrc(kv.k + uniform(row), 0, 16 * hs * ES, 0x00027000);
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s)
-        kr[n][s] = *(const u32x4 *)(at + (uint32_t)(k_row + min(s * M::STEP + kd, k_last) * ES));
+      for (int s = 0; s < STEPS; ++s) {
+        const uint32_t off = FULL ? k_off + s * M::STEP * ES : k_off + min(s * M::STEP + kd, k_last) * ES;
+        kr[n][s] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(at, off, 0, 0));
+      }
     };
     auto load_v = [&](int n, int64_t row) {
-      const char *at = kv.v + uniform(row);
+      const auto at = __builtin_amdgcn_make_buffer_rsrc(kv.v + uniform(row), 0, 16 * hs * ES, 0x00027000);
 #pragma unroll
       for (int s = 0; s < VS; ++s)
 #pragma unroll
-        for (int r = 0; r < RW; ++r) vr[n][s][r] = *(const u32x4 *)(at + (uint32_t)(v_off + s * RS * hs * ES) + 16 * r);
+        for (int r = 0; r < RW; ++r)
+          vr[n][s][r] = __builtin_bit_cast(
+              u32x4, __builtin_amdgcn_raw_buffer_load_b128(at, v_off + 16 * r, s * RS * hs * ES, 0));
     };
 
-    int pids = load_pages(wa), pids_next = load_pages(wa + 64);
+    int pids = pids0, pids_next = load_pages(wa + 64);
     int page[NG], nextp[NG];
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
@@ -300,6 +272,56 @@ __global__ __launch_bounds__(256, split_per_cu(TYPE, HS, GT)) void k_paged_split
       if (wa < wb) load_k(n, at);
       if (wa < wb) load_v(n, at);
     }
+    // ---- the queries as A operands, while the first tile is on its way
+    __syncthreads();  // the last segment's sums have been read
+#pragma unroll
+    for (int s = 0; s < SETS; ++s) {
+      const int h = 4 * s + wid;
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[s][i] *= f;
+        top = fmaxf(top, __builtin_fabsf(x[s][i]));
+      }
+      top = lanes16_max(top, lane);
+      top = fmaxf(top, __uint_as_float(partner_u32<16>(__float_as_uint(top), lane)));
+      top = fmaxf(top, __uint_as_float(partner_u32<32>(__float_as_uint(top), lane)));
+      float to, bk;
+      split_scale<TYPE>(top, to, bk);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[s][i] *= to;
+      if (lane == 0) back[h] = bk;
+      if (8 * lane < HS) {
+        const int row = 4 * wid;
+        if constexpr (TYPE == T_F32) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int d = 8 * lane + 4 * half, at = s * STEPS + d / 16, l0 = (d % 16) / 4 * 16 + row;
+            u32x4 w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(x[s][4 * half + i]);
+            qop[at][l0] = w;
+#pragma unroll
+            for (int r = 1; r < 4; ++r) qop[at][l0 + r] = u32x4{0, 0, 0, 0};
+          }
+        } else {
+          const int at = s * STEPS + lane / 4, l0 = (lane & 3) * 16 + row;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            u32x4 w = {0, 0, 0, 0};
+            if (r < 3)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) w[i] = take_part<TYPE>(x[s][2 * i], x[s][2 * i + 1]);
+            qop[at][l0 + r] = w;
+          }
+        }
+      }
+    }
+    __syncthreads();
+    float bk[SETS];
+#pragma unroll
+    for (int s = 0; s < SETS; ++s) bk[s] = back[s * 4 + kq];
+
     for (int i0 = wa; i0 < wb; i0 += NG) {
       const int nx = i0 + NG - wa;  // the next tile
       if ((nx & 63) == 0) {
@@ -436,91 +458,138 @@ __global__ __launch_bounds__(256, split_per_cu(TYPE, HS, GT)) void k_paged_split
 
     // ---- the four waves joined
 #pragma unroll
-    for (int h = 0; h < GT; ++h)
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int d = LS; d < 64; d <<= 1) acc[h][i] += __shfl_xor(acc[h][i], d, 64);
-#pragma unroll
     for (int s = 0; s < SETS; ++s) l[s] = lanes_sum<16>(l[s], lane);
-    __syncthreads();  // everyone is done with the queries, whose memory this is
+    if (key == 0)
+#pragma unroll
+      for (int s = 0; s < SETS; ++s)
+        if (s * 4 + kq < GT) sm[wid][s * 4 + kq] = m[s], sl[wid][s * 4 + kq] = l[s];
+    __syncthreads();  // and everyone is done with the queries, whose memory the sums take
+    {
+      const int h = lane % GT;  // lane h: head h
+      const float m0 = sm[0][h], m1 = sm[1][h], m2 = sm[2][h], m3 = sm[3][h];
+      const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+      const float mine = shrink(wid < 2 ? (wid == 0 ? m0 : m1) : (wid == 2 ? m2 : m3), top);
+      if (wid == 0 && lane < GT) {
+        stat[h][0] = top;
+        stat[h][1] = ((sl[0][h] * shrink(m0, top) + sl[1][h] * shrink(m1, top)) + sl[2][h] * shrink(m2, top)) +
+                     sl[3][h] * shrink(m3, top);
+      }
+#pragma unroll
+      for (int g = 0; g < GT; ++g) {
+        const float c = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), g));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float v = acc[g][i] * c;
+          if constexpr (LS <= 8) v = add_partner<8>(v, lane);
+          if constexpr (LS <= 16) v = add_partner<16>(v, lane);
+          if constexpr (LS <= 32) v = add_partner<32>(v, lane);
+          acc[g][i] = v;
+        }
+        formed(acc[g]);
+      }
+    }
     if (rl == 0)
 #pragma unroll
       for (int h = 0; h < GT; ++h)
 #pragma unroll
         for (int i = 0; i < 8; i += 4)
           *(float4 *)&so[wid][h][8 * ql + i] = make_float4(acc[h][i], acc[h][i + 1], acc[h][i + 2], acc[h][i + 3]);
-    if (key == 0)
-#pragma unroll
-      for (int s = 0; s < SETS; ++s)
-        if (s * 4 + kq < GT) sm[wid][s * 4 + kq] = m[s], sl[wid][s * 4 + kq] = l[s];
     __syncthreads();
     const bool whole = gi0 == 0 && gi1 == cnt;
     const int64_t slot = 2 * (int64_t)blockIdx.x + (u != begin);
-    for (int i = tid; i < heads * hs; i += 256) {
-      const int h = i / hs, d = i - h * hs;
-      const float top = fmaxf(fmaxf(sm[0][h], sm[1][h]), fmaxf(sm[2][h], sm[3][h]));
-      float o = 0.f, sum = 0.f;
+    float *const out = whole ? a.out + ((int64_t)e * a.n_heads + kvh * group + h0) * hs : pl.part + slot * GT * hs;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float x = shrink(sm[w][h], top);
-        o = __builtin_fmaf(so[w][h][d], x, o);
-        sum = __builtin_fmaf(sl[w][h], x, sum);
+    for (int h = 0; h < GT; ++h) {
+      if (h >= heads) break;
+      const float sum = stat[h][1];
+      const float by = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+      for (int d = 4 * tid; d < hs; d += 1024) {
+        const float4 o0 = *(const float4 *)&so[0][h][d], o1 = *(const float4 *)&so[1][h][d];
+        const float4 o2 = *(const float4 *)&so[2][h][d], o3 = *(const float4 *)&so[3][h][d];
+        float4 o = make_float4(((o0.x + o1.x) + o2.x) + o3.x, ((o0.y + o1.y) + o2.y) + o3.y, ((o0.z + o1.z) + o2.z) + o3.z,
+                               ((o0.w + o1.w) + o2.w) + o3.w);
+        if (whole && sum == 0.f) o = make_float4(0, 0, 0, 0);
+        *(float4 *)(out + (int64_t)h * hs + d) = make_float4(o.x * by, o.y * by, o.z * by, o.w * by);
       }
-      if (whole) {
-        a.out[((int64_t)e * a.n_heads + kvh * group + h0 + h) * hs + d] = sum == 0.f ? 0.f : o / sum;
-      } else {
-        pl.part[(slot * GT + h) * hs + d] = o;
-        if (d == 0) pl.ml[(slot * GT + h) * 2] = top, pl.ml[(slot * GT + h) * 2 + 1] = sum;
-      }
+    }
+    if (!whole && tid < heads) {
+      pl.ml[(slot * GT + tid) * 2] = stat[tid][0];
+      pl.ml[(slot * GT + tid) * 2 + 1] = stat[tid][1];
     }
     u += gi1 - gi0;
   }
 }
 
-// The slots of a head: workgroup (row * n_heads + head, 64 elements), wave w takes slots
-// w, w + 4, ... in order, and the four sums are added in wave order.
-__global__ __launch_bounds__(256) void k_paged_join(PagedArgs a, SplitPlan pl) {
-  __shared__ float ws[4][64], top4[4], sum4[4];
+// The slots of a head: workgroup (row * n_heads + head, 4 ls elements).  64 slots at a time,
+// each wave forms all their weights, a lane each; the slots' values go around the waves,
+// 64 / ls slots to a load, and the waves' sums are added in wave order.
+__global__ __launch_bounds__(256) void k_paged_join(PagedArgs a, SplitPlan pl, int ls) {
+  __shared__ float4 ws[4][64];
   const KvArgs &kv = a.kv;
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int e = blockIdx.x / a.n_heads, h = blockIdx.x - e * a.n_heads;
-  if (*kv.status != KV_OK) return;
-  const int cnt = pl.count[e];
-  if (cnt == 0) return;
+  const int status = *kv.status, cnt = pl.count[e];
+  const int64_t total = pl.first[a.n], before = pl.first[e];
+  if (status != KV_OK || cnt == 0) return;
   const int group = a.n_heads / kv.n_kv, kvh = h / group, hg = h - kvh * group;
-  const int64_t per = stretch_of(pl.first[a.n], pl.wgs);
-  const int64_t ua = pl.first[e] + (int64_t)(kvh * pl.parts + hg / pl.gt) * cnt;
-  const int w0 = (int)(ua / per), w1 = (int)((ua + cnt - 1) / per);
+  const int64_t per = stretch_of(total, pl.wgs, a.n * kv.n_kv * pl.parts);
+  const int64_t ua = before + (int64_t)(kvh * pl.parts + hg / pl.gt) * cnt;
+  const int w0 = (int)quotient(ua, per), w1 = (int)quotient(ua + cnt - 1, per);
   if (w0 == w1) return;
   const int n = w1 - w0 + 1, g = hg % pl.gt;
   const int64_t s0 = 2 * (int64_t)w0 + (ua != w0 * per);  // the first slot; the others are first slots of their stretch
   auto slot = [&](int i) { return (i == 0 ? s0 : 2 * (int64_t)(w0 + i)) * pl.gt + g; };
-  float top = -__builtin_inff();
-  for (int i = tid; i < n; i += 256) top = fmaxf(top, pl.ml[slot(i) * 2]);
-  top = lanes16_max(top, lane);
-  top = fmaxf(top, __uint_as_float(partner_u32<16>(__float_as_uint(top), lane)));
-  top = fmaxf(top, __uint_as_float(partner_u32<32>(__float_as_uint(top), lane)));
-  if (lane == 0) top4[wid] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
-  const int d = blockIdx.y * 64 + lane;
-  const bool live = d < kv.hs;
-  float o = 0.f, sum = 0.f;
-#pragma unroll 8
-  for (int i = wid; i < n; i += 4) {
-    const int64_t s = slot(i);
-    const float x = shrink(pl.ml[s * 2], top);
-    sum = __builtin_fmaf(pl.ml[s * 2 + 1], x, sum);
-    o = __builtin_fmaf(live ? pl.part[s * kv.hs + d] : 0.f, x, o);
+  const int rows = 64 / ls, sub = lane / ls, d = 4 * (blockIdx.y * ls + lane % ls);
+  const float *part = pl.part + (d < kv.hs ? d : 0);
+  float4 o = make_float4(0, 0, 0, 0);
+  float sum = 0.f, top = -__builtin_inff();
+  constexpr int U = 8;
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    const float2 ml = *(const float2 *)(pl.ml + slot(min(i0 + lane, n - 1)) * 2);
+    float c = 1.f, x = 0.f;
+    for (int k0 = 0; k0 < 64; k0 += 4 * U * rows) {
+      if (i0 + k0 >= n) break;
+      float4 v[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        v[k] = make_float4(0, 0, 0, 0);
+        const int i = i0 + k0 + (4 * k + wid) * rows;
+        if (i < n && i < i0 + 64) v[k] = *(const float4 *)(part + slot(min(i + sub, n - 1)) * kv.hs);
+      }
+      if (k0 == 0) {
+        const float m = i0 + lane < n ? ml.x : -__builtin_inff();
+        float t = lanes16_max(m, lane);
+        t = fmaxf(t, __uint_as_float(partner_u32<16>(__float_as_uint(t), lane)));
+        t = fmaxf(t, __uint_as_float(partner_u32<32>(__float_as_uint(t), lane)));
+        t = fmaxf(t, top);
+        c = shrink(top, t), x = shrink(m, t);
+        top = t;
+        sum = __builtin_fmaf(sum, c, x * ml.y);
+        o = make_float4(o.x * c, o.y * c, o.z * c, o.w * c);
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int at = k0 + (4 * k + wid) * rows;
+        if (at >= 64 || i0 + at >= n) break;
+        const float w = __shfl(x, at + sub);  // 0 behind the last slot
+        o.x = __builtin_fmaf(v[k].x, w, o.x), o.y = __builtin_fmaf(v[k].y, w, o.y);
+        o.z = __builtin_fmaf(v[k].z, w, o.z), o.w = __builtin_fmaf(v[k].w, w, o.w);
+      }
+    }
   }
+  for (int s = ls; s < 64; s <<= 1)
+    o.x += __shfl_xor(o.x, s), o.y += __shfl_xor(o.y, s), o.z += __shfl_xor(o.z, s), o.w += __shfl_xor(o.w, s);
   ws[wid][lane] = o;
-  if (lane == 0) sum4[wid] = sum;
+  sum = lanes_sum<64>(sum, lane);
   __syncthreads();
-  if (wid == 0 && live) {
-    const float all = ((sum4[0] + sum4[1]) + sum4[2]) + sum4[3];
-    o = ((ws[0][lane] + ws[1][lane]) + ws[2][lane]) + ws[3][lane];
-    a.out[((int64_t)e * a.n_heads + h) * kv.hs + d] = all == 0.f ? 0.f : o / all;
+  if (wid == 0 && sub == 0 && d < kv.hs) {
+    for (int w = 1; w < 4; ++w) {
+      const float4 v = ws[w][lane];
+      o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+    }
+    const float by = sum == 0.f ? 0.f : 1.f / sum;
+    o = make_float4(o.x * by, o.y * by, o.z * by, o.w * by);
+    *(float4 *)(a.out + ((int64_t)e * a.n_heads + h) * kv.hs + d) = sum == 0.f ? make_float4(0, 0, 0, 0) : o;
   }
 }
 
@@ -547,12 +616,18 @@ static size_t split_layout(const PagedArgs &a, const DevInfo &dev, char *base, S
   return off;
 }
 
+template <int TYPE, int HS, int GT>
+static void launch_split(const PagedArgs &a, const SplitPlan &p, hipStream_t s) {
+  const size_t lds = 8 * (size_t)(a.n + 1) + 12 * (size_t)a.n;
+  if (a.kv.hs == HS) hipLaunchKernelGGL((k_paged_split<TYPE, HS, GT, true>), dim3(p.wgs), dim3(256), lds, s, a, p);
+  else hipLaunchKernelGGL((k_paged_split<TYPE, HS, GT, false>), dim3(p.wgs), dim3(256), lds, s, a, p);
+}
+
 template <int TYPE, int HS>
 static void launch_split(const PagedArgs &a, const SplitPlan &p, hipStream_t s) {
-  const size_t lds = 8 * (size_t)(a.n + 1) + 8 * (size_t)a.n;
-  if (p.gt == 2) hipLaunchKernelGGL((k_paged_split<TYPE, HS, 2>), dim3(p.wgs), dim3(256), lds, s, a, p);
-  else if (p.gt == 4) hipLaunchKernelGGL((k_paged_split<TYPE, HS, 4>), dim3(p.wgs), dim3(256), lds, s, a, p);
-  else hipLaunchKernelGGL((k_paged_split<TYPE, HS, 8>), dim3(p.wgs), dim3(256), lds, s, a, p);
+  if (p.gt == 2) launch_split<TYPE, HS, 2>(a, p, s);
+  else if (p.gt == 4) launch_split<TYPE, HS, 4>(a, p, s);
+  else launch_split<TYPE, HS, 8>(a, p, s);
 }
 
 template <int TYPE>
@@ -576,7 +651,11 @@ hipError_t launch_paged(const PagedArgs &a, const DevInfo &dev, char *scratch, h
   else launch_split<T_BF16>(a, p, s);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(k_paged_join, dim3(a.n * a.n_heads, (a.kv.hs + 63) / 64), dim3(256), 0, s, a, p);
+  int ls = 64;
+  while (ls > 1 && ls * 2 >= a.kv.hs) ls >>= 1;
+  // Heads of many slots are read by more workgroups, or a few CUs would have all of it to read.
+  if (p.wgs > 16 * a.n * a.kv.n_kv * p.parts) ls = ls < 16 ? ls : 16;
+  hipLaunchKernelGGL(k_paged_join, dim3(a.n * a.n_heads, (a.kv.hs + 4 * ls - 1) / (4 * ls)), dim3(256), 0, s, a, p, ls);
   return hipGetLastError();
 }
 

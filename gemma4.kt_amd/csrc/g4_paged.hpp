@@ -54,14 +54,28 @@ struct Raw8 {
   }
 };
 
+// v + the value of lane ^ S; for S = 16 and 32 one swap gives both sides in every lane
+template <int S>
+G4_DEV float add_partner(float v, int lane) {
+  if constexpr (S == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  } else if constexpr (S == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  } else {
+    return v + __uint_as_float(partner_u32<S>(__float_as_uint(v), lane));
+  }
+}
+
 template <int N>
 G4_DEV float lanes_sum(float s, int lane) {  // over each aligned group of N lanes, in every lane of it
-  if constexpr (N > 1) s += __uint_as_float(partner_u32<1>(__float_as_uint(s), lane));
-  if constexpr (N > 2) s += __uint_as_float(partner_u32<2>(__float_as_uint(s), lane));
-  if constexpr (N > 4) s += __uint_as_float(partner_u32<4>(__float_as_uint(s), lane));
-  if constexpr (N > 8) s += __uint_as_float(partner_u32<8>(__float_as_uint(s), lane));
-  if constexpr (N > 16) s += __uint_as_float(partner_u32<16>(__float_as_uint(s), lane));
-  if constexpr (N > 32) s += __uint_as_float(partner_u32<32>(__float_as_uint(s), lane));
+  if constexpr (N > 1) s = add_partner<1>(s, lane);
+  if constexpr (N > 2) s = add_partner<2>(s, lane);
+  if constexpr (N > 4) s = add_partner<4>(s, lane);
+  if constexpr (N > 8) s = add_partner<8>(s, lane);
+  if constexpr (N > 16) s = add_partner<16>(s, lane);
+  if constexpr (N > 32) s = add_partner<32>(s, lane);
   return s;
 }
 
