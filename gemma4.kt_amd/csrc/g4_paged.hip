@@ -67,11 +67,6 @@ struct SplitPlan {
   int32_t gt;
 };
 
-// a / b for a >= 0, b > 0; long division only where the numbers are long
-G4_DEV int64_t quotient(int64_t a, int64_t b) {
-  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
-}
-
 // Units of a stretch: an equal share, but at least a group for each of a workgroup's four
 // waves, where heads have that many.
 G4_DEV int64_t stretch_of(int64_t total, int wgs, int heads) {

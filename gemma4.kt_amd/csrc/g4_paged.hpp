@@ -54,6 +54,11 @@ struct Raw8 {
   }
 };
 
+// a / b for a >= 0, b > 0; long division only where the numbers are long
+G4_DEV int64_t quotient(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 // v + the value of lane ^ S; for S = 16 and 32 one swap gives both sides in every lane
 template <int S>
 G4_DEV float add_partner(float v, int lane) {

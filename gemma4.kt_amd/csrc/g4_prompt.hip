@@ -43,10 +43,10 @@ struct PromptTile {
 
 struct PromptPlan {
   int32_t *n_tiles;   // query tiles of a kv head part
-  int64_t *total;     // their key tiles
-  int32_t *start;     // [wgs] the query tile that a stretch begins in
+  int64_t *total;     // their key tiles, and those of a stretch
+  int32_t *start;     // [wgs][2] the query tile and the unit (kv head part) that a stretch begins in
   PromptTile *tiles;  // [cap]
-  uint16_t *odd;      // [cap][units][bm / 16] rows whose sums are not finite
+  uint16_t *odd;      // [cap][units][bm / 16] rows whose sums are not finite, of tiles in one stretch
   float *part;        // [2 * wgs][bm][hs]
   float *ml;          // [2 * wgs][bm][2]
   int32_t cap;
@@ -92,16 +92,17 @@ G4_DEV KeyTiles key_tiles(int p0, int p1, int window, int sinks, int kt) {
 
 // Key tiles of a stretch.
 G4_DEV int64_t prompt_stretch(int64_t total, int wgs) {
-  const int64_t per = (total + wgs - 1) / wgs;
+  const int64_t per = quotient(total + wgs - 1, wgs);
   return per < 1 ? 1 : per;
 }
 
-// The last tile whose first key tile is <= rel.
-G4_DEV int find_tile(const PromptTile *tiles, int n, int64_t rel) {
+// The last of n ascending numbers (the first is 0) that is not above x.
+template <typename F>
+G4_DEV int last_not_above(F at, int n, int64_t x) {
   int lo = 0, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (tiles[mid].first <= rel) lo = mid;
+    if (at(mid) <= x) lo = mid;
     else hi = mid - 1;
   }
   return lo;
@@ -110,16 +111,17 @@ G4_DEV int find_tile(const PromptTile *tiles, int n, int64_t rel) {
 // One workgroup: the query tiles of every sequence in order, with their key tiles, and
 // the tile that each stretch begins in.
 __global__ __launch_bounds__(1024) void k_prompt_plan(PagedArgs a, PromptPlan pl) {
-  __shared__ int tiles[1025], wsum[16];
-  __shared__ int64_t wsum64[16];
+  __shared__ int tiles[1025], wsum[16], rows[1024], ends[1024], seqs[1024], lens[1024];
+  __shared__ int64_t wsum64[16], firsts[1024];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  if (*a.kv.status != KV_OK) return;
+  const int status = *a.kv.status;  // looked at once the rest is here too
   int mine = 0;
   if (tid < a.n) {
-    int from, to;
-    entry_rows(a, tid, from, to);
-    mine = (to - from + pl.tt - 1) / pl.tt;
+    entry_rows(a, tid, rows[tid], ends[tid]);
+    lens[tid] = entry_length(a, tid, seqs[tid]);
+    mine = (ends[tid] - rows[tid] + pl.tt - 1) / pl.tt;
   }
+  if (status != KV_OK) return;
   int x = mine;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -144,10 +146,8 @@ __global__ __launch_bounds__(1024) void k_prompt_plan(PagedArgs a, PromptPlan pl
         if (tiles[mid] <= t) lo = mid;
         else hi = mid - 1;
       }
-      int from, to;
-      entry_rows(a, lo, from, to);
-      const int tok = (t - tiles[lo]) * pl.tt;
-      it.len = entry_length(a, lo, it.seq);
+      const int from = rows[lo], to = ends[lo], tok = (t - tiles[lo]) * pl.tt;
+      it.len = lens[lo], it.seq = seqs[lo];
       it.row = from + tok;
       it.toks = min(pl.tt, to - it.row);
       it.base = it.len - (to - from) + tok;
@@ -169,17 +169,25 @@ __global__ __launch_bounds__(1024) void k_prompt_plan(PagedArgs a, PromptPlan pl
     if (t < n_tiles) {
       it.first = mybase + s - it.count;
       pl.tiles[t] = it;
+      if (t0 == 0) firsts[t] = it.first;
     }
     before += all;
     __syncthreads();
   }
-  if (tid == 0) *pl.n_tiles = n_tiles, *pl.total = before;
-  if (before == 0) return;
-  __threadfence_block();  // the tiles, for the search
-  __syncthreads();
   const int64_t all = before * a.kv.n_kv * pl.parts, per = prompt_stretch(all, pl.wgs);
-  for (int w = tid; w < pl.wgs; w += 1024)
-    if (w * per < all) pl.start[w] = find_tile(pl.tiles, n_tiles, w * per % before);
+  if (tid == 0) *pl.n_tiles = n_tiles, pl.total[0] = before, pl.total[1] = per;
+  if (before == 0) return;
+  if (n_tiles > 1024) {
+    __threadfence_block();  // the tiles, for the search
+    __syncthreads();
+  }
+  for (int w = tid; w < pl.wgs; w += 1024) {
+    if (w * per >= all) break;
+    const int64_t hu = quotient(w * per, before), rel = w * per - hu * before;
+    pl.start[2 * w + 1] = (int)hu;
+    pl.start[2 * w] = n_tiles > 1024 ? last_not_above([&](int i) { return pl.tiles[i].first; }, n_tiles, rel)
+                                     : last_not_above([&](int i) { return firsts[i]; }, n_tiles, rel);
+  }
 }
 
 // 16 bytes a lane from src (the same in all lanes) + off to LDS at `to` + 16 * lane.
@@ -233,11 +241,10 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), hs = kv.hs;
   if (*kv.status != KV_OK) return;
   const int group = a.n_heads / kv.n_kv, units = kv.n_kv * pl.parts, n_tiles = *pl.n_tiles;
-  const int64_t per_unit = *pl.total, total = per_unit * units;
+  const int64_t per_unit = pl.total[0], per = pl.total[1], total = per_unit * units;
 
   // Workgroups b, b + 8, ... run on one XCD: they take neighbouring stretches, so that
   // the key tiles of a kv head are read into few L2s.
-  const int64_t per = prompt_stretch(total, pl.wgs);
   const int stretch = pl.wgs % 8 == 0 ? (blockIdx.x & 7) * (pl.wgs >> 3) + (blockIdx.x >> 3) : blockIdx.x;
   const int64_t begin = stretch * per, end = min(total, begin + per);
 
@@ -247,7 +254,7 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
   const int64_t layer_rows = (int64_t)a.layer * kv.n_pages * kv.n_kv << kv.shift;
 
   if (begin >= end) return;
-  int tile = __builtin_amdgcn_readfirstlane(pl.start[stretch]), hu = (int)(begin / per_unit);
+  int tile = __builtin_amdgcn_readfirstlane(pl.start[2 * stretch]), hu = __builtin_amdgcn_readfirstlane(pl.start[2 * stretch + 1]);
   for (int64_t u = begin; u < end; ++tile) {
     if (tile == n_tiles) tile = 0, ++hu;
     const PromptTile it = pl.tiles[tile];
@@ -711,12 +718,13 @@ __global__ __launch_bounds__(256) void k_paged_prompt_join(PagedArgs a, PromptPl
   __shared__ float sm[4 * 8], sl[4 * 8], so[4 * HS];
   __shared__ int32_t bad[16];
   const KvArgs &kv = a.kv;
-  const int tid = threadIdx.x, hs = kv.hs, words = hs / 4;
-  if (*kv.status != KV_OK) return;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hs = kv.hs, words = hs / 4;
   const int units = kv.n_kv * pl.parts, tile = blockIdx.x / units, hu = blockIdx.x - tile * units;
-  if (tile >= *pl.n_tiles) return;
-  const PromptTile it = pl.tiles[tile];
-  const int64_t per_unit = *pl.total, per = prompt_stretch(per_unit * units, pl.wgs);
+  const int status = *kv.status, n_tiles = *pl.n_tiles;
+  const PromptTile it = pl.tiles[tile];  // inside the table, if behind the last tile
+  const int64_t per_unit = pl.total[0], per = pl.total[1];
+  if (status != KV_OK || tile >= n_tiles) return;
   const int group = a.n_heads / kv.n_kv, kvh = hu / pl.parts, h0 = (hu - kvh * pl.parts) * pl.gh;
   const int heads = min(pl.gh, group - h0), r0 = blockIdx.y * 16, r1 = min(r0 + 16, it.toks * heads);
   if (r0 >= r1) return;
@@ -731,38 +739,82 @@ __global__ __launch_bounds__(256) void k_paged_prompt_join(PagedArgs a, PromptPl
     return;
   }
   const int64_t ua = hu * per_unit + it.first;
-  const int w0 = (int)(ua / per), w1 = (int)((ua + it.count - 1) / per);
-  if (tid < 16) bad[tid] = 0;
-  __syncthreads();
-  if (w0 != w1) {
+  const int w0 = (int)quotient(ua, per), w1 = (int)quotient(ua + it.count - 1, per);
+  if (w0 == w1) {
+    const uint32_t odd = pl.odd[(int64_t)blockIdx.x * (pl.bm / 16) + blockIdx.y];
+    if (odd == 0) return;
+    if (tid < 16) bad[tid] = odd >> tid & 1;
+    __syncthreads();
+  } else {
+    const int n = w1 - w0 + 1, rw = r0 + 4 * wid;  // slots, and the first of the wave's four rows
     const int64_t s0 = 2 * (int64_t)w0 + (ua != w0 * per);
-    for (int i = tid; i < (r1 - r0) * words; i += 256) {
-      const int r = r0 + i / words, x = i % words;
-      float top = -__builtin_inff();
-#pragma unroll 4
-      for (int w = w0; w <= w1; ++w) top = fmaxf(top, pl.ml[((w == w0 ? s0 : 2 * (int64_t)w) * pl.bm + r) * 2]);
-      float4 o = make_float4(0, 0, 0, 0);
-      float sum = 0.f;
-#pragma unroll 4
-      for (int w = w0; w <= w1; ++w) {
-        const int64_t at = (w == w0 ? s0 : 2 * (int64_t)w) * pl.bm + r;
-        const float c = shrink(pl.ml[at * 2], top);
-        const float4 v = *(const float4 *)(pl.part + at * hs + 4 * x);
-        sum = __builtin_fmaf(pl.ml[at * 2 + 1], c, sum);
-        o.x = __builtin_fmaf(v.x, c, o.x), o.y = __builtin_fmaf(v.y, c, o.y);
-        o.z = __builtin_fmaf(v.z, c, o.z), o.w = __builtin_fmaf(v.w, c, o.w);
+    auto slot = [&](int i) { return (i == 0 ? s0 : 2 * (int64_t)(w0 + i)) * pl.bm; };
+    auto row = [&](int j) { return min(rw + j, r1 - 1); };
+    if (tid < 16) bad[tid] = 0;
+    __syncthreads();
+    for (int d0 = 0; d0 < hs; d0 += 256) {
+      const int d = d0 + 4 * lane;
+      const float *part = pl.part + (d < hs ? d : 0);
+      float4 o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = make_float4(0, 0, 0, 0);
+      float top = -__builtin_inff(), sum = 0.f;  // of row lane / 16
+      for (int i0 = 0; i0 < n; i0 += 16) {
+        const int mine = i0 + (lane & 15);
+        const float2 ml = *(const float2 *)(pl.ml + (slot(min(mine, n - 1)) + row(lane >> 4)) * 2);
+        float x = 0.f;
+        for (int k0 = 0; k0 < 16; k0 += 4) {
+          if (i0 + k0 >= n) break;
+          float4 v[4][4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (i0 + k0 + k < n) {
+              const int64_t at = slot(i0 + k0 + k);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) v[k][j] = *(const float4 *)(part + (at + row(j)) * hs);
+            }
+          }
+          if (k0 == 0) {
+            const float m = mine < n ? ml.x : -__builtin_inff();
+            const float t = fmaxf(top, lanes16_max(m, lane)), c = shrink(top, t);
+            x = shrink(m, t);
+            top = t;
+            sum = __builtin_fmaf(sum, c, mine < n ? x * ml.y : 0.f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float cj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(c), 16 * j));
+              o[j] = make_float4(o[j].x * cj, o[j].y * cj, o[j].z * cj, o[j].w * cj);
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (i0 + k0 + k < n) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 16 * j + k0 + k));
+                o[j].x = __builtin_fmaf(v[k][j].x, w, o[j].x), o[j].y = __builtin_fmaf(v[k][j].y, w, o[j].y);
+                o[j].z = __builtin_fmaf(v[k][j].z, w, o[j].z), o[j].w = __builtin_fmaf(v[k][j].w, w, o[j].w);
+              }
+            }
+          }
+        }
       }
-      const bool none = sum == 0.f;
-      o.x = none ? 0.f : o.x / sum, o.y = none ? 0.f : o.y / sum, o.z = none ? 0.f : o.z / sum, o.w = none ? 0.f : o.w / sum;
-      *(float4 *)(a.out + out_at(r, tk) * hs + 4 * x) = o;
-      if (!(__builtin_fabsf(o.x) < __builtin_inff()) || !(__builtin_fabsf(o.y) < __builtin_inff()) ||
-          !(__builtin_fabsf(o.z) < __builtin_inff()) || !(__builtin_fabsf(o.w) < __builtin_inff()))
-        bad[r - r0] = 1;
+      sum = lanes_sum<16>(sum, lane);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float s = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sum), 16 * j));
+        if (rw + j >= r1 || d >= hs) continue;
+        const bool none = s == 0.f;
+        const float4 y = make_float4(none ? 0.f : o[j].x / s, none ? 0.f : o[j].y / s, none ? 0.f : o[j].z / s,
+                                     none ? 0.f : o[j].w / s);
+        *(float4 *)(a.out + out_at(rw + j, tk) * hs + d) = y;
+        if (!(__builtin_fabsf(y.x) < __builtin_inff()) || !(__builtin_fabsf(y.y) < __builtin_inff()) ||
+            !(__builtin_fabsf(y.z) < __builtin_inff()) || !(__builtin_fabsf(y.w) < __builtin_inff()))
+          bad[rw + j - r0] = 1;
+      }
     }
-  } else if (tid < r1 - r0) {
-    bad[tid] = pl.odd[(int64_t)blockIdx.x * (pl.bm / 16) + blockIdx.y] >> tid & 1;
+    __syncthreads();
   }
-  __syncthreads();
   for (int r = r0; r < r1; ++r) {
     if (!bad[r - r0]) continue;
     const int64_t at = out_at(r, tk);
@@ -789,8 +841,8 @@ static size_t prompt_layout(const PagedArgs &a, const DevInfo &dev, char *base, 
   };
   const size_t cap = (size_t)p->cap, units = (size_t)a.kv.n_kv * p->parts;
   p->n_tiles = (int32_t *)add(4);
-  p->total = (int64_t *)add(8);
-  p->start = (int32_t *)add(4 * (size_t)p->wgs);
+  p->total = (int64_t *)add(16);
+  p->start = (int32_t *)add(8 * (size_t)p->wgs);
   p->tiles = (PromptTile *)add(sizeof(PromptTile) * cap);
   p->odd = (uint16_t *)add(2 * cap * units * (p->bm / 16));
   p->part = (float *)add(sizeof(float) * 2 * (size_t)p->wgs * p->bm * a.kv.hs);
@@ -809,8 +861,7 @@ static hipError_t launch_tiles(const PagedArgs &a, const PromptPlan &p, hipStrea
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   constexpr int JHS = HS == 96 ? 128 : HS == 192 ? 256 : HS;
-  hipLaunchKernelGGL((k_paged_prompt_join<TYPE, JHS>), dim3(p.cap * a.kv.n_kv * p.parts, p.bm / 16), dim3(256), 0, s,
-                     a, p);
+  hipLaunchKernelGGL((k_paged_prompt_join<TYPE, JHS>), dim3(p.cap * a.kv.n_kv * p.parts, p.bm / 16), dim3(256), 0, s, a, p);
   return hipGetLastError();
 }
 
