@@ -1751,6 +1751,11 @@ int check_rope(const g4_rope *r, int32_t head_size, g4::RopeArgs *a) {
   return G4_OK;
 }
 
+// Ranges of `bytes` that share memory, but are not the same one.
+bool half_overlap(const void *a, const void *b, size_t bytes) {
+  return a != b && (const char *)a < (const char *)b + bytes && (const char *)b < (const char *)a + bytes;
+}
+
 int kv_move(g4_ctx *ctx, const g4_kv *kv, g4::KvMove m, const char *what) {
   g4::KvArgs a;
   G4_TRY(check_kv(kv, &a));
@@ -1929,6 +1934,8 @@ int g4_rope_dev(g4_ctx *ctx, const g4_rope *rope, const float *d_x, float *d_out
   G4_TRY(check_rope(rope, head_size, &r));
   if (n_rows == 0) return G4_OK;
   if (!d_x || !d_out || !d_positions) return fail(G4_ERR_INVALID_ARGUMENT, "null pointer");
+  if (half_overlap(d_x, d_out, sizeof(float) * (size_t)n_rows * n_heads * head_size))
+    return fail(G4_ERR_INVALID_ARGUMENT, "x and out overlap");
   G4_TRY(use_device(ctx));
   return launch_status(g4::launch_rope(r, d_x, d_out, n_rows, n_heads, head_size, d_positions, ctx->stream), "rope");
 }
@@ -1951,6 +1958,8 @@ int g4_kv_rope_write_dev(g4_ctx *ctx, const g4_kv *kv, int32_t layer, const g4_r
   if (rope) G4_TRY(check_rope(rope, kv->head_size, &r));
   if (n == 0 || n_rows == 0) return G4_OK;
   if (!d_k || !d_v) return fail(G4_ERR_INVALID_ARGUMENT, "null pointer");
+  if (d_q && half_overlap(d_q, d_q_out, sizeof(float) * (size_t)n_rows * n_heads * kv->head_size))
+    return fail(G4_ERR_INVALID_ARGUMENT, "q and q_out overlap");
   G4_TRY(use_device(ctx));
   const g4::KvWrite w = {layer, d_q, d_q_out, d_k, d_v, d_q ? n_heads : 0, n, d_seqs, d_row_begin, n_rows};
   return launch_status(g4::launch_kv_write(a, r, w, ctx->stream), "cache write");

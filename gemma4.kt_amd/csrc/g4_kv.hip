@@ -546,56 +546,74 @@ template <int TYPE, int N>
 __global__ __launch_bounds__(256) void k_kv_write(KvArgs kv, RopeArgs r, KvWrite w) {
   __shared__ int begin[KV_MAX_SEQS];
   const int row = blockIdx.x, tid = threadIdx.x;
-  if (*kv.status != KV_OK) return;
+  const int status = *kv.status;
+  const int units = kv.hs / (2 * N), slots = 256 / units, slot = tid / units, u = tid % units;
+  const int heads = w.n_heads + 2 * kv.n_kv;
+  const int per = (heads + gridDim.y - 1) / gridDim.y;
+  const int h0 = blockIdx.y * per, h1 = slot < slots ? min(heads, h0 + per) : 0;
+  int a, b;
+  bool turn;
+  unit_at<N>(r, u, a, b, turn);
+  float x[N], y[N];
+  auto load = [&](int h) {
+    const float *from = h < w.n_heads ? w.q + ((int64_t)row * w.n_heads + h) * kv.hs
+                        : h < w.n_heads + kv.n_kv
+                            ? w.k + ((int64_t)row * kv.n_kv + h - w.n_heads) * kv.hs
+                            : w.v + ((int64_t)row * kv.n_kv + h - w.n_heads - kv.n_kv) * kv.hs;
+    load_floats<N>(from + a, x);
+    load_floats<N>(from + b, y);
+  };
+  if (h0 + slot < h1) load(h0 + slot);  // on its way while the row's place is looked up
+  if (status != KV_OK) return;
   int e = row, rows = 1, at = 0;
+  bool bad = false;
   if (w.row_begin) {
-    for (int i = tid; i < w.n; i += 256) begin[i] = w.row_begin[i];
-    __syncthreads();
-    if (row < begin[0] || row >= w.row_begin[w.n]) return;  // behind the last sequence: left as it is
+    for (int i = tid; i < w.n; i += 256) {
+      const int from = w.row_begin[i], to = w.row_begin[i + 1];
+      bad |= from < 0 || to < from || to > w.n_rows;
+      begin[i] = from;
+    }
+    const int last = w.row_begin[w.n];
+    if (__syncthreads_or(bad)) {
+      if (tid == 0) atomicCAS(kv.status, KV_OK, KV_BAD_DATA);
+      return;
+    }
+    if (row < begin[0] || row >= last) return;  // behind the last sequence: left as it is
     e = find_entry(begin, w.n, row);
     rows = w.row_begin[e + 1] - begin[e];
     at = row - begin[e];
   }
   const int seq = w.seqs[e], len = safe_length(kv, seq);
+  for (int i = tid; i < w.n; i += 256) bad |= i != e && w.seqs[i] == seq;  // two rows for one place
   const int pos = len - rows + at;
   int page = -1;
   if (pos >= 0 && pos < len) page = kv.table[(int64_t)seq * kv.max_pages + (pos >> kv.shift)];
+  float c[N], s[N];
+  if (turn && h0 + slot < min(h1, w.n_heads + kv.n_kv))
+#pragma unroll
+    for (int i = 0; i < N; ++i) turn_of((double)pos, r.freqs[u * N + i], r.gain, c[i], s[i]);
   // the page is there, and no other sequence holds it
-  if (!in_range(page, kv.n_pages) || kv.refs[page] != 1) {
+  bad |= !in_range(page, kv.n_pages) || kv.refs[page] != 1;
+  if (__syncthreads_or(bad)) {
     if (tid == 0) atomicCAS(kv.status, KV_OK, KV_BAD_DATA);
     return;
   }
-  const int units = kv.hs / (2 * N), slots = 256 / units, slot = tid / units, u = tid % units;
-  const int heads = w.n_heads + 2 * kv.n_kv;
-  const int per = (heads + gridDim.y - 1) / gridDim.y;
-  const int h0 = blockIdx.y * per, h1 = min(heads, h0 + per);
-  if (slot >= slots) return;
-  int a, b;
-  bool turn;
-  unit_at<N>(r, u, a, b, turn);
-  float c[N], s[N];
-  if (turn && h0 + slot < w.n_heads + kv.n_kv)
-#pragma unroll
-    for (int i = 0; i < N; ++i) turn_of((double)pos, r.freqs[u * N + i], r.gain, c[i], s[i]);
-  for (int h = h0 + slot; h < h1; h += slots) {
+  for (int h = h0 + slot; h < h1;) {
     const bool is_q = h < w.n_heads, is_k = !is_q && h < w.n_heads + kv.n_kv;
-    const int kh = is_k ? h - w.n_heads : h - w.n_heads - kv.n_kv;
-    const float *from = is_q ? w.q + ((int64_t)row * w.n_heads + h) * kv.hs
-                             : (is_k ? w.k : w.v) + ((int64_t)row * kv.n_kv + kh) * kv.hs;
-    float x[N], y[N];
-    load_floats<N>(from + a, x);
-    load_floats<N>(from + b, y);
     rotate<N>(turn && (is_q || is_k), r.pairs, c, s, x, y);
     if (is_q) {
       float *to = w.q_out + ((int64_t)row * w.n_heads + h) * kv.hs;
       store_as<T_F32, N>((char *)to, a, x);
       store_as<T_F32, N>((char *)to, b, y);
     } else {
+      const int kh = is_k ? h - w.n_heads : h - w.n_heads - kv.n_kv;
       const int64_t at_page = ((((int64_t)w.layer * kv.n_pages + page) * kv.n_kv + kh) * kv.page + (pos & (kv.page - 1))) *
                               (int64_t)kv.hs;
       store_as<TYPE, N>(is_k ? kv.k : kv.v, at_page + a, x);
       store_as<TYPE, N>(is_k ? kv.k : kv.v, at_page + b, y);
     }
+    h += slots;
+    if (h < h1) load(h);
   }
 }
 

@@ -58,12 +58,6 @@ struct PromptPlan {
   int32_t tt;         // tokens of a query tile
 };
 
-// Rows of entry e, inside the call's whatever row_begin holds.
-G4_DEV void entry_rows(const PagedArgs &a, int e, int &from, int &to) {
-  from = min(max(a.row_begin[e], 0), a.n_rows);
-  to = min(max(a.row_begin[e + 1], from), a.n_rows);
-}
-
 // Length and number of its sequence.
 G4_DEV int entry_length(const PagedArgs &a, int e, int &seq) {
   seq = a.seqs[e];
@@ -116,12 +110,19 @@ __global__ __launch_bounds__(1024) void k_prompt_plan(PagedArgs a, PromptPlan pl
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const int status = *a.kv.status;  // looked at once the rest is here too
   int mine = 0;
+  bool bad = false;
   if (tid < a.n) {
-    entry_rows(a, tid, rows[tid], ends[tid]);
+    const int from = a.row_begin[tid], to = a.row_begin[tid + 1];
+    bad = from < 0 || to < from || to > a.n_rows;  // rising, or there were more tiles than the table holds
+    rows[tid] = from, ends[tid] = to;
     lens[tid] = entry_length(a, tid, seqs[tid]);
-    mine = (ends[tid] - rows[tid] + pl.tt - 1) / pl.tt;
+    mine = bad ? 0 : (to - from + pl.tt - 1) / pl.tt;
   }
   if (status != KV_OK) return;
+  if (__syncthreads_or(bad)) {
+    if (tid == 0) *a.kv.status = KV_BAD_DATA;
+    return;
+  }
   int x = mine;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -134,7 +135,7 @@ __global__ __launch_bounds__(1024) void k_prompt_plan(PagedArgs a, PromptPlan pl
   tiles[tid + 1] = x;
   if (tid == 0) tiles[0] = 0;
   __syncthreads();
-  const int n_tiles = min(tiles[a.n], pl.cap);
+  const int n_tiles = tiles[a.n];  // at most cap
   int64_t before = 0;
   for (int t0 = 0; t0 < n_tiles; t0 += 1024) {
     const int t = t0 + tid;

@@ -395,8 +395,9 @@ int g4_rope_dev(g4_ctx *ctx, const g4_rope *rope, const float *d_x, float *d_out
  * queries), d_k [n_rows][n_kv_heads][head_size] is turned and d_v taken as it is, and
  * both are written to the sequence's pages, rounded to nearest (F16 overflows to
  * infinity).  rope NULL: nothing is turned, and d_q is NULL.  Rows of no sequence
- * are left as they are.  A row whose page is not there or is shared is not written,
- * and *status is set.  A sequence is named once.  One launch. */
+ * are left as they are.  A row whose page is not there or is shared, or whose sequence is
+ * named twice, is not written, and *status is set; no row is if d_row_begin does not
+ * rise.  One launch. */
 int g4_kv_rope_write_dev(g4_ctx *ctx, const g4_kv *kv, int32_t layer, const g4_rope *rope, const float *d_q,
                          float *d_q_out, const float *d_k, const float *d_v, int32_t n_heads, int32_t n,
                          const int32_t *d_seqs, const int32_t *d_row_begin, int32_t n_rows);
@@ -409,13 +410,14 @@ int g4_kv_rope_write_dev(g4_ctx *ctx, const g4_kv *kv, int32_t layer, const g4_r
  * over the tokens t <= p that it sees: all (window = 0), or t > p - window and the
  * first `sinks`.  A row that sees nothing (an empty sequence, pages given back, scores
  * that are all -infinity) is zeros.  fp32 products and sums.  d_q and d_out are 16-byte
- * aligned and do not overlap. */
+ * aligned and do not overlap.  Two launches. */
 int g4_paged_attention_dev(g4_ctx *ctx, const g4_kv *kv, int32_t layer, const float *d_q, float *d_out,
                            int32_t n_heads, int32_t n, const int32_t *d_seqs, float scale, int32_t window,
                            int32_t sinks);
 /* The same for several tokens per sequence (prompts, their chunks, drafted tokens): the
  * rows of each sequence as in g4_kv_rope_write_dev, each at its own position and seeing
- * no later one.  Rows of no sequence are left as they are. */
+ * no later one.  Rows of no sequence are left as they are; if d_row_begin does not rise,
+ * all are, and *status is set.  Three launches. */
 int g4_paged_prompt_dev(g4_ctx *ctx, const g4_kv *kv, int32_t layer, const float *d_q, float *d_out, int32_t n_heads,
                         int32_t n, const int32_t *d_seqs, const int32_t *d_row_begin, int32_t n_rows, float scale,
                         int32_t window, int32_t sinks);

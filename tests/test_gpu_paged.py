@@ -743,3 +743,150 @@ def test_results_do_not_depend_on_what_ran_before(g4, run):
         outs.append((a, b))
     for a, b in outs[1:]:
         assert torch.equal(a, outs[0][0]) and torch.equal(b, outs[0][1])
+
+
+# ----------------------------------------------------- calls at their edges ---
+
+def test_write_refuses_a_sequence_named_twice(g4, run):
+    """Two rows for one place: neither is written; the other sequences' rows are."""
+    announce("a sequence twice")
+    cache = filled(g4, run, 70, "f16", 1, 2, 64, 16, [20, 9, 33], garbage=0.0)
+    before = Model(cache)
+    k = torch.ones(3, 2, 64, device="cuda")
+    g4.kv_rope_write_dev(run, cache, 0, None, None, k, k, 0, None, i32([2, 1, 2]), None, 3)
+    with pytest.raises(g4.IndexOutOfBoundsException):
+        g4.kv_status(run, cache)
+    page = int(before.table[2, 2])
+    for mine, theirs in ((before.k, cache.k.cpu()), (before.v, cache.v.cpu())):
+        assert torch.equal(mine[0, page].view(torch.int16), theirs[0, page].view(torch.int16))
+    g4.kv_rope_write_dev(run, cache, 0, None, None, k, k, 0, None, i32([0, 0]), i32([0, 1, 3]), 3)
+    with pytest.raises(g4.IndexOutOfBoundsException):
+        g4.kv_status(run, cache)
+
+
+@pytest.mark.parametrize("begin,rows", [([0, 5, 3, 9], 9), ([-1, 2, 4, 9], 9), ([0, 4, 8, 12], 9)], ids=str)
+def test_rows_that_do_not_rise(g4, run, begin, rows):
+    """Refused on the device: nothing is written, the cache says so."""
+    announce("row_begin %s" % begin)
+    cache = filled(g4, run, 71, "bf16", 1, 2, 64, 16, [20, 9, 33], garbage=0.0)
+    before = Model(cache)
+    q = torch.randn(rows, 4, 64, device="cuda")
+    out = torch.full_like(q, 7.0)
+    k = torch.ones(rows, 2, 64, device="cuda")
+    for call in (lambda: g4.paged_prompt_dev(run, cache, 0, q, out, 4, i32([0, 1, 2]), i32(begin), rows, 0.1),
+                 lambda: g4.kv_rope_write_dev(run, cache, 0, None, None, k, k, 0, None, i32([0, 1, 2]), i32(begin), rows)):
+        call()
+        with pytest.raises(g4.IndexOutOfBoundsException):
+            g4.kv_status(run, cache)
+    assert bool((out == 7.0).all())
+    before.same_contents(cache)
+
+
+@pytest.mark.parametrize("typ,heads,hs", [("f16", 16, 512), ("f32", 8, 512), ("bf16", 3, 64)], ids=str)
+def test_the_longest_list(g4, run, typ, heads, hs):
+    """1024 entries, sequences named many times, decode and prompt; the prompt's single
+    rows against decode of the same."""
+    announce("1024 entries, %s, %d heads of %d" % (typ, heads, hs))
+    cache = filled(g4, run, 72, typ, 1, 1, hs, 16, [70, 1, 0, 16, 33, 200])
+    model = Model(cache)
+    order = [int(x) for x in torch.randint(0, 6, (1024,), generator=gen(73))]
+    q = normal(gen(74), 1024, heads, hs).cuda()
+    out, again = torch.empty_like(q), torch.empty_like(q)
+    scale = hs ** -0.5
+    g4.paged_attention_dev(run, cache, 0, q, out, heads, i32(order), scale, 40, 3)
+    g4.paged_prompt_dev(run, cache, 0, q, again, heads, i32(order), i32(range(1025)), 1024, scale, 40, 3)
+    torch.cuda.synchronize()
+    rows = list(range(0, 1024, 61)) + [1022, 1023]
+    for o in (out, again):
+        check_rows(o, [(r, order[r], int(model.lengths[order[r]]) - 1) for r in rows], model, 0, q, scale, 40, 3)
+    # the largest bound of a value is 1 sigma * 5 and the mean: rows of both differ by less than twice 1e-5 of it
+    assert float((out - again).abs().max()) <= 2e-5 * 10
+
+
+def test_offsets_beyond_32_bits(g4, run):
+    """A cache of 9.7 GB a side: pages behind 4 GB and behind 2^31 elements give the bits of
+    the same pages in a small cache."""
+    announce("a large cache")
+    kv, hs, page, pages, heads = 8, 512, 256, 1160, 16
+    big = g4.KvCache.create(run, 2, kv, hs, page, pages, 2, 8, torch.float32)
+    small = g4.KvCache.create(run, 2, kv, hs, page, 6, 2, 8, torch.float32)
+    assert big.k[0].numel() > 1 << 30 and big.k.numel() > 1 << 31
+    g = gen(75)
+    far = [pages - 1, pages - 7, pages - 400, pages - 2, 700, pages - 3]
+    length = 2 * page + 37
+    for i, p in enumerate(far[:3]):
+        for a, b in ((small.k, big.k), (small.v, big.v)):
+            rows = normal(g, 2, kv, page, hs).cuda()
+            a[:, i] = rows
+            b[:, p] = rows
+    big.refs.fill_(9)  # none is free but the ones below
+    for c, ids in ((small, range(6)), (big, far)):
+        ids = list(ids)
+        c.table[0, :3] = i32(ids[:3])
+        c.refs[i32(ids[:3]).long()] = 1
+        c.refs[i32(ids[3:]).long()] = 0
+        c.lengths[0] = length
+    q1, qn = normal(g, 1, heads, hs).cuda(), normal(g, 300, heads, hs).cuda()
+    k, v = normal(g, 5, kv, hs).cuda(), normal(g, 5, kv, hs).cuda()
+    outs = []
+    for c in (small, big):
+        o1, on = torch.empty_like(q1), torch.empty_like(qn)
+        g4.kv_extend_dev(run, c, i32([0]), i32([5]))
+        g4.kv_rope_write_dev(run, c, 1, None, None, k, v, 0, None, i32([0]), i32([0, 5]), 5)
+        g4.kv_fork_dev(run, c, i32([0]), i32([1]))
+        g4.paged_attention_dev(run, c, 1, q1, o1, heads, i32([1]), 0.04)
+        g4.paged_prompt_dev(run, c, 1, qn, on, heads, i32([1]), i32([0, 300]), 300, 0.04)
+        assert g4.kv_status(run, c) is None
+        outs.append((o1, on))
+    assert int(big.table[1, 2]) == min(700, pages - 3) and big.table[1, :2].tolist() == far[:2]
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+    assert torch.equal(big.k[:, 700, :, :42], big.k[:, far[2], :, :42])
+
+
+def test_two_graphs_share_a_context(g4, ctx):
+    """Decode and prompt recorded into two graphs over one workspace, replayed in turn with
+    eager calls between, each replay against the eager result."""
+    announce("two graphs")
+    c2 = g4.Context(0)
+    try:
+        c2.reserve(128 << 20)
+        one = filled(g4, c2, 76, "bf16", 1, 2, 128, 16, [1500, 40, 700])
+        two = filled(g4, c2, 77, "f16", 1, 4, 64, 32, [900, 333])
+        q, p = normal(gen(78), 3, 8, 128).cuda(), normal(gen(79), 500, 8, 64).cuda()
+        a, b = torch.empty_like(q), torch.empty_like(p)
+        s1, s2, begin = i32([2, 0, 1]), i32([1, 0]), i32([0, 100, 500])
+
+        def decode(out):
+            g4.paged_attention_dev(c2, one, 0, q, out, 8, s1, 0.1, 900, 4)
+
+        def prompt(out):
+            g4.paged_prompt_dev(c2, two, 0, p, out, 8, s2, begin, 500, 0.1)
+
+        torch.cuda.synchronize()
+        graphs, stream = [], torch.cuda.Stream()
+        for body, out in ((decode, a), (prompt, b)):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                c2.set_stream(stream.cuda_stream)
+                body(out)
+            c2.set_stream(None)
+            graphs.append(graph)
+        g = gen(80)
+        for i in range(6):
+            for t in (q, p):
+                t.copy_(normal(g, *t.shape))
+            a.fill_(float("nan"))
+            b.fill_(float("nan"))
+            torch.cuda.synchronize()
+            for j in (0, 1) if i % 2 else (1, 0, 1):
+                graphs[j].replay()
+            torch.cuda.synchronize()
+            ea, eb = torch.empty_like(a), torch.empty_like(b)
+            torch.cuda.synchronize()
+            prompt(eb)
+            decode(ea)
+            c2.sync()
+            assert torch.equal(a, ea) and torch.equal(b, eb)
+    finally:
+        torch.cuda.synchronize()
+        c2.close()

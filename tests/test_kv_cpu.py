@@ -241,3 +241,18 @@ def test_wrappers_refuse_what_is_not_on_the_device():
                  lambda: g4hip.paged_prompt_dev(ctx, cache, 0, f, f, 2, i, i, 4)):
         with pytest.raises(g4hip.IllegalArgumentException):
             call()
+
+
+def test_overlapping_rotations_are_refused(hip):
+    """In place or apart: a result that begins inside its operand would be read half turned."""
+    with Program(hip) as p:
+        s = struct()
+        r = g4hip._RopeStruct(4096, 64, 0, 1.0)
+        at, rope, c = ctypes.addressof(s), ctypes.addressof(r), p.ctx
+        size = 2 * 4 * 128 * 4  # 2 rows of 4 heads of 128 floats
+        for off, want in ((0, 0), (16, INVALID), (-16, INVALID), (size - 16, INVALID), (size, 0), (-size, 0)):
+            assert hip.g4_rope_dev(c, rope, 1 << 20, (1 << 20) + off, 2, 4, 128, 4096) == want
+        size = 3 * 8 * s.head_size * 4
+        for off, want in ((0, 0), (16, INVALID), (-16, INVALID), (size - 16, INVALID), (size, 0)):
+            assert hip.g4_kv_rope_write_dev(c, at, 0, rope, 1 << 20, (1 << 20) + off, 4096, 4096, 8, 3, 4096, None,
+                                            3) == want
