@@ -22,27 +22,46 @@ constexpr int KV_T = 1024;  // threads of the bookkeeping workgroup, one per lis
 
 static_assert(KV_T >= KV_MAX_SEQS, "one thread per entry");
 
-// Exclusive sum over a workgroup of KV_T threads; *total is everyone's sum.  `ws`: one
-// int per wave.  Ends with a barrier, so that ws can be used again.
-G4_DEV int block_scan(int v, int *ws, int *total) {
+// Inclusive sum over a wave: by 1, 2, 4 and 8 lanes inside rows of 16, then the last lane
+// of a row to the next, and of the first two rows to the last two.
+G4_DEV int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+  return x;
+}
+
+// Exclusive sums of N numbers over a workgroup of KV_T threads; total: everyone's.  `ws`:
+// N ints per wave.  Ends with a barrier, so that ws can be used again.
+template <int N>
+G4_DEV void block_scan(int (&v)[N], int *ws, int (&total)[N]) {
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  int x = v;
+  int x[N], mine[N];
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d, 64);
-    if (lane >= d) x += y;
-  }
-  if (lane == 63) ws[wid] = x;
-  __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < KV_T / 64; ++w) {
-    const int s = ws[w];
-    if (w < wid) before += s;
-    all += s;
+  for (int i = 0; i < N; ++i) {
+    x[i] = wave_scan(v[i]);
+    if (lane == 63) ws[N * wid + i] = x[i];
   }
   __syncthreads();
-  *total = all;
-  return before + x - v;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {  // a lane for each wave
+    const int t = wave_scan(lane < KV_T / 64 ? ws[N * lane + i] : 0);
+    total[i] = __builtin_amdgcn_readlane(t, KV_T / 64 - 1);
+    mine[i] = wid ? __shfl(t, wid - 1) : 0;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = mine[i] + x[i] - v[i];
+}
+
+G4_DEV int block_scan(int v, int *ws, int *total) {
+  int a[1] = {v}, t[1];
+  block_scan(a, ws, t);
+  *total = t[0];
+  return a[0];
 }
 
 G4_DEV int64_t block_sum_i64(int64_t v, int64_t *ws) {
@@ -75,28 +94,35 @@ G4_DEV int find_entry(const int *begin, int n, int x) {
   return lo;
 }
 
-// Calls give(rank, page) for the `total` lowest free pages, from a whole workgroup.
-// Returns the number found, at most total.
-template <class F>
-G4_DEV int lowest_free(const KvArgs &kv, int total, int *ws, F give) {
+// Which of a thread's four pages from `base` on are free: bit j for page base + 4 thread + j.
+G4_DEV int four_free(const KvArgs &kv, int64_t base) {
   typedef int32_t i32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
+  const int64_t p0 = base + 4 * (int64_t)threadIdx.x;
+  int f = 0;
+  if (p0 + 4 <= kv.n_pages) {
+    const i32x4a4 r = *(const i32x4a4 *)(kv.refs + p0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f |= (r[j] == 0) << j;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f |= (p0 + j < kv.n_pages && kv.refs[p0 + j] == 0) << j;
+  }
+  return f;
+}
+
+// Calls give(rank, page) for the `total` lowest free pages, from a whole workgroup.
+// Returns the number found, at most total.  f: four_free(kv, 0).
+template <class F>
+G4_DEV int lowest_free(const KvArgs &kv, int total, int *ws, int f, F give) {
   int found = 0;
   for (int64_t base = 0; base < kv.n_pages && found < total; base += 4 * KV_T) {
-    const int64_t p0 = base + 4 * (int64_t)threadIdx.x;
-    int f[4];
-    if (p0 + 4 <= kv.n_pages) {
-      const i32x4a4 r = *(const i32x4a4 *)(kv.refs + p0);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) f[j] = r[j] == 0;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) f[j] = p0 + j < kv.n_pages && kv.refs[p0 + j] == 0;
-    }
-    int all, rank = found + block_scan(f[0] + f[1] + f[2] + f[3], ws, &all);
+    if (base > 0) f = four_free(kv, base);
+    const int p0 = (int)base + 4 * threadIdx.x;
+    int all, rank = found + block_scan(__builtin_popcount(f), ws, &all);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (f[j]) {
-        if (rank < total) give(rank, (int)(p0 + j));
+      if (f >> j & 1) {
+        if (rank < total) give(rank, p0 + j);
         ++rank;
       }
     found += all;
@@ -114,7 +140,8 @@ __global__ __launch_bounds__(256) void k_kv_init(KvArgs kv) {
   if (i == 0) *kv.status = KV_OK;
 }
 
-// lengths[seqs[i]] += counts[i], with the pages that takes.
+// lengths[seqs[i]] += counts[i], with the pages that takes.  The free pages are found
+// by counting refs, 4096 at a time: latency, as in k_kv_plan.
 __global__ __launch_bounds__(KV_T) void k_kv_extend(KvArgs kv, int n, const int32_t *seqs, const int32_t *counts) {
   __shared__ int mark[KV_MAX_SEQS], first[KV_T + 1], row[KV_T], have[KV_T], ws[KV_T / 64];
   __shared__ int64_t ws64[KV_T / 64];
@@ -151,12 +178,13 @@ __global__ __launch_bounds__(KV_T) void k_kv_extend(KvArgs kv, int n, const int3
   __syncthreads();
   // the pages are counted before the first is given out
   if (total64 > 0) {
-    const int found = total64 > kv.n_pages ? 0 : lowest_free(kv, total, ws, [](int, int) {});
+    const int free4 = four_free(kv, 0);
+    const int found = total64 > kv.n_pages ? 0 : lowest_free(kv, total, ws, free4, [](int, int) {});
     if (found < total64) {
       if (tid == 0) *kv.status = KV_NO_PAGES;
       return;
     }
-    lowest_free(kv, total, ws, [&](int rank, int page) {
+    lowest_free(kv, total, ws, free4, [&](int rank, int page) {
       const int e = find_entry(first, n, rank);
       kv.table[(int64_t)row[e] * kv.max_pages + have[e] + rank - first[e]] = page;
       kv.refs[page] = 1;
@@ -248,7 +276,8 @@ size_t kv_move_scratch_bytes(const KvArgs &kv, const KvMove &m) {
   return plan_layout(kv, m, nullptr, &p);
 }
 
-// Where each listed token is.
+// Where each listed token is: two dependent loads each, 5 us for 18000 tokens, which one
+// workgroup (k_kv_plan's) would take 18 rounds for.
 __global__ __launch_bounds__(KV_RES) void k_kv_resolve(KvArgs kv, KvMove m, Plan p) {
   __shared__ int begin[KV_MAX_SEQS];
   if (*kv.status != KV_OK) return;
@@ -270,18 +299,22 @@ __global__ __launch_bounds__(KV_RES) void k_kv_resolve(KvArgs kv, KvMove m, Plan
   if (threadIdx.x == 0) p.bad[blockIdx.x] = any;
 }
 
+// Checks the call, counts what it needs and lists the fresh pages.  One workgroup: 5 us
+// for 64 entries and 4000 pages, of which a launch is 2; its loads depend on each other
+// (lists, lengths, table, refs).  Sums by lane permutes and two counts a barrier took it
+// from 6.5 us.
 __global__ __launch_bounds__(KV_T) void k_kv_plan(KvArgs kv, KvMove m, Plan p) {
-  __shared__ int mark[KV_MAX_SEQS], ws[KV_T / 64];
-  __shared__ int64_t ws64[KV_T / 64];
-  const int tid = threadIdx.x;
-  if (*kv.status != KV_OK) {
+  __shared__ int mark[KV_MAX_SEQS], ws[2 * KV_T / 64];
+  const int tid = threadIdx.x, status = *kv.status;
+  const int free4 = four_free(kv, 0);  // on its way while the lists are read
+  mark[tid] = 0;
+  bool bad = false;
+  for (int i = tid; i < p.n_bad; i += KV_T) bad |= p.bad[i] != 0;
+  __syncthreads();
+  if (status != KV_OK) {
     if (tid == 0) *p.ok = 0;
     return;
   }
-  mark[tid] = 0;
-  __syncthreads();
-  bool bad = false;
-  for (int i = tid; i < p.n_bad; i += KV_T) bad |= p.bad[i] != 0;
   int prefix = 0, shared = 0, length = 0, need = 0, copies = 0, src_page = -1;
   if (tid < m.n) {
     const int src = m.src[tid], dst = m.dst[tid];
@@ -317,32 +350,33 @@ __global__ __launch_bounds__(KV_T) void k_kv_plan(KvArgs kv, KvMove m, Plan p) {
     if (tid == 0) *kv.status = KV_BAD_DATA, *p.ok = 0;
     return;
   }
-  // every count below is at most n_keep + n * page, which the host has checked
-  const int64_t total64 = block_sum_i64(need, ws64);
-  int total, all;
-  const int f = block_scan(need, ws, &total);
-  const int c = block_scan(copies, ws, &all);
+  // The lists of kept tokens follow each other, so the copies are at most n_keep + n * page,
+  // which the host has checked, and the pages fewer.
+  int sums[2] = {need, copies}, all[2];
+  block_scan(sums, ws, all);
   if (tid < m.n) {
     p.prefix[tid] = prefix;
     p.shared[tid] = shared;
     p.length[tid] = length;
     p.src_page[tid] = src_page;
-    p.fresh_begin[tid] = f;
-    p.copy_begin[tid] = c;
+    p.fresh_begin[tid] = sums[0];
+    p.copy_begin[tid] = sums[1];
   }
-  if (tid == 0) p.fresh_begin[m.n] = total, p.copy_begin[m.n] = all;
+  if (tid == 0) p.fresh_begin[m.n] = all[0], p.copy_begin[m.n] = all[1];
   int found = 0;
-  if (total64 <= p.fresh_cap)
-    found = lowest_free(kv, total, ws, [&](int rank, int page) { p.fresh[rank] = page; });
+  if (all[0] <= p.fresh_cap)
+    found = lowest_free(kv, all[0], ws, free4, [&](int rank, int page) { p.fresh[rank] = page; });
   if (tid == 0) {
-    *p.ok = found == total64;
-    if (found != total64) *kv.status = KV_NO_PAGES;
+    *p.ok = found == all[0];
+    if (found != all[0]) *kv.status = KV_NO_PAGES;
   }
 }
 
 // The copies (workgroups below n_copy: `per` tokens of one layer each), and the new
 // rows of the table, 16 columns a workgroup: every old row is read before one is
-// written, since a sequence can be another's source.
+// written, since a sequence can be another's source.  Bound by memory: 64 forks of 16
+// prompts copy 55 MB in 23.5 us (4.7 TB/s read and written; a large copy reaches 5.1),
+// tokens kept out of 16 sequences 169 MB in 74 us (4.6 TB/s, rows of 256 bytes).
 constexpr int KV_COLS = 16;
 
 __global__ __launch_bounds__(256) void k_kv_move(KvArgs kv, KvMove m, Plan p, int n_copy, int per) {
@@ -541,7 +575,10 @@ G4_DEV void rotate(bool turn, bool pairs, const float (&c)[N], const float (&s)[
 // A workgroup turns a stretch of the heads of one row (blockIdx.x; blockIdx.y of
 // gridDim.y stretches): thread (slot, u) takes unit u of every slots-th head and so
 // forms its cosines once.  Heads 0 .. n_heads - 1 are q, then n_kv of k, then n_kv of v.
-// It is bound by memory for prompts and by latency for single rows.
+// Bound by memory for prompts (8000 rows of 32/4 heads of 128, F16: 64 us, 4.8 TB/s of the
+// 5.1 that a copy reaches) and by latency for single rows (32 of them 7.5 us: the row's
+// sequence, its length, page and owner are four loads that wait for each other, and its
+// first head comes meanwhile).
 template <int TYPE, int N>
 __global__ __launch_bounds__(256) void k_kv_write(KvArgs kv, RopeArgs r, KvWrite w) {
   __shared__ int begin[KV_MAX_SEQS];
@@ -617,6 +654,7 @@ __global__ __launch_bounds__(256) void k_kv_write(KvArgs kv, RopeArgs r, KvWrite
   }
 }
 
+// Rows at given positions, as k_kv_write turns them; bound by memory.
 template <int N>
 __global__ __launch_bounds__(256) void k_rope(RopeArgs r, const float *x, float *out, int n_heads, int hs,
                                               const int32_t *positions) {

@@ -18,16 +18,31 @@ namespace g4 {
 // in order, are cut into equal stretches, one per workgroup, whatever the lengths are:
 // they are device data, which each workgroup sums up itself.  Where a stretch holds all
 // of a head's groups the result is final; otherwise (maximum, sum, weighted values) goes
-// to the stretch's first or second slot and k_paged_join adds the slots of a head.
+// to the stretch's first or second slot and k_paged_join adds the slots of a head.  One
+// workgroup per (row, kv head, pair of query heads) left the chip to the longest row: it
+// took 936 us for the 64 rows below and 580 us for the one of 8192 tokens.
 //
 // A wave takes NG groups at a time.  Scores come from the matrix cores: A = the query
 // heads, B = 16 keys as they lie in memory.  A head is four rows of A: for a 16-bit
 // cache the query's three 16-bit parts, which add up to it exactly, for F32 the query
 // itself; the products are then exact (F32: rounded once), and a lane's sum over its
 // four rows of C is the score of (head lane / 16, key lane % 16).  The queries carry
-// scale * log2(e) (split_scale keeps their parts in range).  Values are weighted by the vector unit in fp32, eight
-// elements of a row per lane, with the weights handed over through the wave's own LDS.
-// While a tile is worked on, the next one's keys and values are on their way.
+// scale * log2(e) (split_scale keeps their parts in range).  Values are weighted by the
+// vector unit in fp32, eight elements of a row per lane, with the weights handed over
+// through the wave's own LDS.  While a tile is worked on, the next one's keys and values
+// are on their way: a wave's registers hold both, and LDS only the queries.
+//
+// What bounds it is the cache's bytes, read once (FETCH_SIZE is 1.00 to 1.09 of K and V),
+// where rows are long, and the chain of loads at a stretch's start (lengths, page table,
+// keys: about 2000 clocks each) where a stretch is a few groups.  Measured, with its join:
+//   4 rows of 20001 to 65536 tokens, 8/2 heads of 256, F32    123 us, 5.3 TB/s
+//   64 rows of 200 to 16384 tokens, 32/4 heads of 128, F16    136 us, 3.6 TB/s: with eight
+//     heads to a kv head the 64 products of a value lane take as long as its loads
+//   1 row of 8192 tokens, 16/8 heads of 256, BF16             20.6 us, 3.3 TB/s
+//   24 rows in a window of 1024, 8/1 heads of 512, BF16       34 us, 1.5 TB/s: two groups a wave
+// (a copy's reads alone reach 5.86 TB/s).  Tiles of twice the groups where one workgroup
+// fills a CU (512 registers a lane) cost 30% on the last: the values pass through
+// accumulation registers.
 
 // A row's visible tokens as groups: the first gs, then those from g0.
 struct Groups {
@@ -517,7 +532,9 @@ __global__ __launch_bounds__(256, split_per_cu(TYPE, HS, GT)) void k_paged_split
 
 // The slots of a head: workgroup (row * n_heads + head, 4 ls elements).  64 slots at a time,
 // each wave forms all their weights, a lane each; the slots' values go around the waves,
-// 64 / ls slots to a load, and the waves' sums are added in wave order.
+// 64 / ls slots to a load, and the waves' sums are added in wave order.  Bound by latency
+// (status, plan, slots, one after the other): 5 us for one row's 64 slots a head, 9 us for
+// 2048 heads of one to three.
 __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a, SplitPlan pl, int ls) {
   __shared__ float4 ws[4][64];
   const KvArgs &kv = a.kv;
@@ -648,7 +665,9 @@ hipError_t launch_paged(const PagedArgs &a, const DevInfo &dev, char *scratch, h
   if (e != hipSuccess) return e;
   int ls = 64;
   while (ls > 1 && ls * 2 >= a.kv.hs) ls >>= 1;
-  // Heads of many slots are read by more workgroups, or a few CUs would have all of it to read.
+  // Heads of many slots are read by more workgroups, or a few CUs would have all of it to
+  // read: 16 heads of 64 slots take 4.8 us, with 256 elements a workgroup 6.8; 2048 heads of
+  // one to three slots 9.0 us that way, and 10.6 with 64 elements.
   if (p.wgs > 16 * a.n * a.kv.n_kv * p.parts) ls = ls < 16 ? ls : 16;
   hipLaunchKernelGGL(k_paged_join, dim3(a.n * a.n_heads, (a.kv.hs + 4 * ls - 1) / (4 * ls)), dim3(256), 0, s, a, p, ls);
   return hipGetLastError();

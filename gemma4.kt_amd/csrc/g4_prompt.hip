@@ -4,8 +4,8 @@
 // Every row is a token of a sequence and a query head; it sees what g4_paged.hip says,
 // causally.  A query tile is up to BM rows of one sequence that share a kv head: its
 // consecutive tokens times the heads of that kv head.  Keys and values come in tiles of
-// KT tokens through LDS (two buffers, loaded straight to LDS while the other is worked
-// on) and are used by all waves; a wave has 16 rows.
+// KT tokens through LDS (two buffers, loaded straight to LDS by half of the waves while
+// the other is worked on) and are used by all waves; a wave has 16 rows.
 //
 // Both products are on the matrix cores, transposed, so that a lane stays with one row
 // (column lane % 16 of every product):
@@ -22,9 +22,27 @@
 // The (kv head, query tile, key tile) units are cut into equal stretches, one per
 // persistent workgroup, whatever the lengths, windows and causal triangles are
 // (k_prompt_plan counts them); a query tile whose key tiles are spread over several
-// stretches leaves (maximum, sum, O) of each in a slot, and k_prompt_join adds them.  A
-// row whose sums are not finite (an infinite or NaN key or value among those it meets,
-// maybe hidden from it) is computed again by k_prompt_join, from the formula.
+// stretches leaves (maximum, sum, O) of each in a slot, and k_paged_prompt_join adds them.
+// A row whose sums are not finite (an infinite or NaN key or value among those it meets,
+// maybe hidden from it) is computed again by k_paged_prompt_join, from the formula: a
+// prompt of nothing but NaN takes 25 times as long as any other.
+//
+// Operands are read from LDS four (BF16) or six products ahead of their use (a read takes
+// 64 clocks alone, more with eight waves reading); two ahead, with all waves loading, took
+// 1417 us for the prompt of 8192 tokens below.
+//
+// What bounds it, and what it measured (times of all three kernels; the products count
+// once, though BF16 takes each three times and F16 twice; a library product of 8192^3 in
+// the same type reaches 1086 and 1029 TFLOP/s on the card):
+//   8192 tokens, causal, 16/8 heads of 256, BF16    1290 us at 2.1 GHz: 427 TFLOP/s, 1.28
+//     PFLOP/s of matrix instructions, 60% of their cycles; the clock falls with them
+//   four chunks of 301 to 1100 rows behind up to 12001 tokens, window 4096, 16/4 heads of 128,
+//     F16    201 us: 361 TFLOP/s; 4.9 vector instructions to a matrix instruction (the
+//     weights of a row are the same work for a head of 128 as for one of 256)
+//   8 sequences of 5 drafted tokens behind 1000 to 16384, 16/8 heads of 256, BF16    101 us,
+//     3.9 TB/s: one wave of eight has rows, and computes as long as a tile's 64 KB take
+//   1001 tokens in a window of 512, 8/2 heads of 256, F16    48 us: three key tiles a
+//     stretch, so mostly its start and end, and the two small kernels
 #include "g4_paged.hpp"
 
 namespace g4 {
@@ -103,7 +121,8 @@ G4_DEV int last_not_above(F at, int n, int64_t x) {
 }
 
 // One workgroup: the query tiles of every sequence in order, with their key tiles, and
-// the tile that each stretch begins in.
+// the tile that each stretch begins in.  5.5 us, all of it latency: two loads that depend on
+// each other, two scans, a search in LDS.
 __global__ __launch_bounds__(1024) void k_prompt_plan(PagedArgs a, PromptPlan pl) {
   __shared__ int tiles[1025], wsum[16], rows[1024], ends[1024], seqs[1024], lens[1024];
   __shared__ int64_t wsum64[16], firsts[1024];
@@ -200,8 +219,8 @@ G4_DEV void load_to_lds(const char *src, uint32_t off, uint32_t to) {
 // The loads to LDS and the LDS operations of the wave are done; then all waves meet.
 G4_DEV void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// Operands read ahead of the product that takes them.
-constexpr int prompt_ahead(int type, int hs) { return type == T_BF16 ? 4 : 6; }
+// Operands read ahead of the product that takes them; BF16's third part leaves fewer registers.
+constexpr int prompt_ahead(int type) { return type == T_BF16 ? 4 : 6; }
 
 constexpr int prompt_waves(int hs) { return hs > 256 ? 4 : 8; }
 constexpr int prompt_kt(int type, int hs) {
@@ -421,7 +440,7 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
         pat[i] = lds0 + buf * 2 * HALF + at_col * ROW + (((4 * i) ^ g4 ^ Z::k(at_col)) << 4);
         asm volatile("" : "+v"(pat[i]));
       }
-      constexpr int N = STEPS * NT, A = prompt_ahead(TYPE, HS);
+      constexpr int N = STEPS * NT, A = prompt_ahead(TYPE);
       u32x4 k[A + 1];
       auto read = [&](int i) {
         const int st = i / NT;
@@ -536,7 +555,7 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
           u32x4 w;
         };
         // 16 elements of the head after the other, over 32 keys a product
-        constexpr int N = ND * NT / 2, A = prompt_ahead(TYPE, HS);
+        constexpr int N = ND * NT / 2, A = prompt_ahead(TYPE);
         Operand v[A + 1];
         uint32_t pat[8];  // as for the keys
 #pragma unroll
@@ -713,7 +732,11 @@ G4_DEV void plain_row(const PagedArgs &a, int64_t at, int kvh, int seq, int pos,
 
 // One workgroup per (query tile, kv head part, 16 rows): adds the slots of a tile whose
 // key tiles were spread over several stretches, in order, computes rows again that are
-// not finite, and writes the zeros of rows that see nothing.
+// not finite, and writes the zeros of rows that see nothing.  A wave has four rows, and
+// their slots' weights a lane each; four slots of four rows are on their way at a time.
+// Bound by latency, and by its 104 registers (four workgroups to a CU): 7.5 us for 64 tiles
+// of 10 rows, 10.5 us for 30 MB of slots.  Workgroups per boundary between stretches,
+// which looked for rows to be done again afterwards, took 2 to 5 us longer.
 template <int TYPE, int HS>
 __global__ __launch_bounds__(256) void k_paged_prompt_join(PagedArgs a, PromptPlan pl) {
   __shared__ float sm[4 * 8], sl[4 * 8], so[4 * HS];
