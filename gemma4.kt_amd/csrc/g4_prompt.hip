@@ -27,18 +27,20 @@
 // maybe hidden from it) is computed again by k_paged_prompt_join, from the formula: a
 // prompt of nothing but NaN takes 25 times as long as any other.
 //
-// Operands are read from LDS four (BF16) or six products ahead of their use (a read takes
-// 64 clocks alone, more with eight waves reading); two ahead, with all waves loading, took
-// 1417 us for the prompt of 8192 tokens below.
+// Operands are read from LDS a few products ahead of their use (a read takes 64 clocks alone,
+// more with eight waves reading).
 //
 // What bounds it, and what it measured (times of all three kernels; the products count
 // once, though BF16 takes each three times and F16 twice; a library product of 8192^3 in
 // the same type reaches 1086 and 1029 TFLOP/s on the card):
-//   8192 tokens, causal, 16/8 heads of 256, BF16    1290 us at 2.1 GHz: 427 TFLOP/s, 1.28
-//     PFLOP/s of matrix instructions, 60% of their cycles; the clock falls with them
+//   8192 tokens, causal, 16/8 heads of 256, BF16    1280 to 1340 us (the clock falls with the
+//     matrix instructions, card by card): 410 to 430 TFLOP/s, 1.2 to 1.3 PFLOP/s of matrix
+//     instructions, 60% of their cycles.  The transposed reads of values are 16% of the time
+//     (441 us for 4096 tokens, 371 with a tile's first operands used throughout)
 //   four chunks of 301 to 1100 rows behind up to 12001 tokens, window 4096, 16/4 heads of 128,
-//     F16    201 us: 361 TFLOP/s; 4.9 vector instructions to a matrix instruction (the
-//     weights of a row are the same work for a head of 128 as for one of 256)
+//     F16    187 us: 388 TFLOP/s; 4.9 vector instructions to a matrix instruction (the
+//     weights of a row are the same work for a head of 128 as for one of 256).  Without any
+//     reads from LDS it would be 177 us
 //   8 sequences of 5 drafted tokens behind 1000 to 16384, 16/8 heads of 256, BF16    101 us,
 //     3.9 TB/s: one wave of eight has rows, and computes as long as a tile's 64 KB take
 //   1001 tokens in a window of 512, 8/2 heads of 256, F16    48 us: three key tiles a
@@ -219,10 +221,18 @@ G4_DEV void load_to_lds(const char *src, uint32_t off, uint32_t to) {
 // The loads to LDS and the LDS operations of the wave are done; then all waves meet.
 G4_DEV void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// Operands read ahead of the product that takes them; BF16's third part leaves fewer registers.
-constexpr int prompt_ahead(int type) { return type == T_BF16 ? 4 : 6; }
+// Operands read ahead of the product that takes them: with four (BF16) or six (F16) 4096 tokens
+// of 16/4 heads of 128 take 257 and 221 us, with three 249 and 219, and BF16 spills fewer registers.
+// F32 takes four products to an operand's 16 elements: six ahead 203 us for 2048 tokens, three 209.
+constexpr int prompt_ahead(int type) { return type == T_F32 ? 6 : 3; }
 
-constexpr int prompt_waves(int hs) { return hs > 256 ? 4 : 8; }
+// Waves of a workgroup: as many as fit a CU with the registers that a row's query, sums and
+// weights take (up to 168 a lane for heads up to 128, 256 up to 256, 512 beyond).  For heads up
+// to 128 a third wave on a SIMD has work where two wait for LDS and exponentials: 4096 tokens of
+// 16/4 heads take 222 us with 12 waves and 247 with 8 for 128 elements in F16, 157 and 188 for
+// 64, 258 and 267 for 128 in BF16 (which spills 4 registers); 16 waves
+// (128 registers) take as long for 64 elements and spill 35 for 128.
+constexpr int prompt_waves(int hs) { return hs > 256 ? 4 : hs <= 128 ? 12 : 8; }
 constexpr int prompt_kt(int type, int hs) {
   const int es = type == T_F32 ? 4 : 2, kt = 32768 / (hs * es);
   return kt > 64 ? 64 : kt >= 64 ? 64 : kt >= 32 ? 32 : 16;
@@ -512,7 +522,8 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
               const auto hi = __builtin_amdgcn_cvt_pkrtz(w0, w1);
               typedef float f32x2 __attribute__((ext_vector_type(2)));
               typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-              const f16x2 lo = __builtin_convertvector((f32x2{w0 - (float)hi[0], w1 - (float)hi[1]}), f16x2);
+              const f16x2 lo = __builtin_convertvector(
+                  (f32x2{__builtin_fmaf((float)hi[0], -1.f, w0), __builtin_fmaf((float)hi[1], -1.f, w1)}), f16x2);
               pb[0][n][i] = __builtin_bit_cast(uint32_t, hi) ^ flip;
               pb[1][n][i] = __builtin_bit_cast(uint32_t, lo) ^ flip;
             } else {
