@@ -653,6 +653,18 @@ G4_DEV void am_step(float &v, int &i, int lane) {
   if (am_better(ov, oi, v, i)) v = ov, i = oi;
 }
 
+// Inclusive sum over a wave: by 1, 2, 4 and 8 lanes inside rows of 16, then the last lane
+// of a row to the next, and of the first two rows to the last two.
+G4_DEV int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+  return x;
+}
+
 // (value, index) arg-max over the 64 lanes of a wave; every lane ends with the result.
 G4_DEV void am_wave(float &v, int &i) {
   const int lane = __lane_id();

@@ -22,18 +22,6 @@ constexpr int KV_T = 1024;  // threads of the bookkeeping workgroup, one per lis
 
 static_assert(KV_T >= KV_MAX_SEQS, "one thread per entry");
 
-// Inclusive sum over a wave: by 1, 2, 4 and 8 lanes inside rows of 16, then the last lane
-// of a row to the next, and of the first two rows to the last two.
-G4_DEV int wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
-  return x;
-}
-
 // Exclusive sums of N numbers over a workgroup of KV_T threads; total: everyone's.  `ws`:
 // N ints per wave.  Ends with a barrier, so that ws can be used again.
 template <int N>

@@ -16,7 +16,9 @@ namespace g4 {
 // are taken in groups of 16 aligned ones, each inside one page; a (row, kv head, up to
 // GT of its query heads) has as many units of work as groups.  The units of all of them,
 // in order, are cut into equal stretches, one per workgroup, whatever the lengths are:
-// they are device data, which each workgroup sums up itself.  Where a stretch holds all
+// they are device data, which each workgroup sums up itself.  Where there are fewer heads than
+// workgroups, stretches end where heads do, if they get little longer by it: a stretch
+// across two heads costs a second start and end.  Where a stretch holds all
 // of a head's groups the result is final; otherwise (maximum, sum, weighted values) goes
 // to the stretch's first or second slot and k_paged_join adds the slots of a head.  One
 // workgroup per (row, kv head, pair of query heads) left the chip to the longest row: it
@@ -38,10 +40,10 @@ namespace g4 {
 //   4 rows of 20001 to 65536 tokens, 8/2 heads of 256, F32    123 us, 5.3 TB/s
 //   64 rows of 200 to 16384 tokens, 32/4 heads of 128, F16    136 us, 3.6 TB/s: with eight
 //     heads to a kv head the 64 products of a value lane take as long as its loads
-//   1 row of 8192 tokens, 16/8 heads of 256, BF16             20.6 us, 3.3 TB/s
-//   24 rows in a window of 1024, 8/1 heads of 512, BF16       34 us, 1.5 TB/s: two groups a wave
+//   1 row of 8192 tokens, 16/8 heads of 256, BF16             21 us, 3.2 TB/s
+//   24 rows in a window of 1024, 8/1 heads of 512, BF16       27 us, 1.9 TB/s: two groups a wave
 // (a copy's reads alone reach 5.86 TB/s).  Tiles of twice the groups where one workgroup
-// fills a CU (512 registers a lane) cost 30% on the last: the values pass through
+// fills a CU (512 registers a lane) took 40% longer on the last: the values pass through
 // accumulation registers.
 
 // A row's visible tokens as groups: the first gs, then those from g0.
@@ -73,7 +75,7 @@ constexpr int split_per_cu(int type, int hs, int gt) {
 
 // Where the stretches and their slots lie.
 struct SplitPlan {
-  int64_t *first;  // [n + 1] units before each row
+  int64_t *first;  // [n + 1] units before each row; then the units of a stretch, and what heads are padded to
   int32_t *count;  // [n] groups of each row
   float *part;     // [2 * wgs][GT][hs]
   float *ml;       // [2 * wgs][GT][2]
@@ -89,6 +91,14 @@ G4_DEV int64_t stretch_of(int64_t total, int wgs, int heads) {
   const int64_t least = mean < 1 ? 1 : mean > 4 ? 4 : mean;
   return per < least ? least : per;
 }
+
+// Groups that a segment's start and end are worth: 15000 clocks of a CU's 10 bytes.
+constexpr int segment_worth(int type, int hs) {
+  const int groups = 150000 / (32 * hs * (type == T_F32 ? 4 : 2));
+  return groups < 4 ? 4 : groups;
+}
+
+G4_DEV int padded(int count, int pad) { return pad == 1 ? count : (count + pad - 1) / pad * pad; }
 
 // A score whose products or sums the matrix cores could not form (an infinite key times
 // a part that is zero, a sum beyond fp32): the dot product as it is written.
@@ -119,6 +129,9 @@ __global__ __launch_bounds__(256, split_per_cu(TYPE, HS, GT)) void k_paged_split
   __shared__ float sm[4][GT], sl[4][GT], stat[GT][2], back[SETS * 4];
   __shared__ int64_t wsum[4];
   extern __shared__ __align__(16) char dyn[];  // first [n + 1], count [n], length [n], sequence [n]
+  int64_t per;
+  int pad = 1;
+  bool aligned = false;
   u32x4(*qop)[64] = (u32x4(*)[64])shared;
   float(*so)[GT][HS] = (float(*)[GT][HS])shared;
   int64_t *first = (int64_t *)dyn;
@@ -148,22 +161,58 @@ __global__ __launch_bounds__(256, split_per_cu(TYPE, HS, GT)) void k_paged_split
         mine += (int64_t)c[j] * units;
       }
     }
-    int64_t x = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t y = __shfl_up(x, d, 64);
-      if (lane >= d) x += y;
+    if (a.n * units <= (int)gridDim.x) {
+      // Stretches that end where heads do, if that makes them no longer than a second segment
+      // would: the shortest of three lengths with which every head's pieces have a workgroup each.
+      // (Sums in 32 bits: of counts cut to 2^21 groups, for the lengths to try only.)
+      // 24 rows in a window of 1024, 8/1 heads of 512, BF16: 27.2 us, 34.4 with equal stretches;
+      // 30 of up to 3000 in a window of 512, 8/2 of 128, F16: 17.4 and 21.5; one row whose heads
+      // fill equal stretches anyway pays 0.3 us for the choice.
+      __syncthreads();
+      auto wave_total = [](int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); };
+      int all = 0;
+      for (int r = lane; r < a.n; r += 64) all += min(count[r], 1 << 21);
+      const int least = (int)stretch_of((int64_t)wave_total(all) * units, gridDim.x, a.n * units);
+      for (int i = 2; i >= 0; --i) {
+        const uint32_t p = least + i * (segment_worth(TYPE, HS) / 2);
+        int pieces = 0;
+        for (int r = lane; r < a.n; r += 64) pieces += min((count[r] + p - 1) / p, 1u << 20);
+        if (wave_total(pieces) > (int)gridDim.x / units) break;
+        pad = p, aligned = true;
+      }
     }
-    if (lane == 63) wsum[wid] = x;
+    // first: sums of 64 bits, or of the heads' pieces, of which there are few
+    int64_t x, step[4];
+    if (aligned) {
+      int few = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) few += c[j] = (int)((uint32_t)(c[j] + pad - 1) / (uint32_t)pad);
+      const int s = wave_scan(few);
+      if (lane == 63) wsum[wid] = s;
+      x = s - few;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) step[j] = c[j];
+    } else {
+      x = mine;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int64_t y = __shfl_up(x, d, 64);
+        if (lane >= d) x += y;
+      }
+      if (lane == 63) wsum[wid] = x;
+      x -= mine;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) step[j] = (int64_t)c[j] * units;
+    }
     __syncthreads();
-    x -= mine;
     for (int w = 0; w < wid; ++w) x += wsum[w];
+    const int64_t each = aligned ? (int64_t)pad * units : 1;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int e = 4 * tid + j;
-      if (e < a.n) first[e] = x;
-      x += (int64_t)c[j] * units;
-      if (e + 1 == a.n) first[a.n] = x;
+      if (e < a.n) first[e] = x * each;
+      x += step[j];
+      if (e + 1 == a.n) first[a.n] = x * each;
     }
     __syncthreads();
   }
@@ -178,7 +227,8 @@ __global__ __launch_bounds__(256, split_per_cu(TYPE, HS, GT)) void k_paged_split
     if (count[e] == 0)
       for (int i = tid; i < a.n_heads * hs; i += 256) a.out[(int64_t)e * a.n_heads * hs + i] = 0.f;
 
-  const int64_t per = stretch_of(first[a.n], gridDim.x, a.n * units);
+  per = aligned ? pad : stretch_of(first[a.n], gridDim.x, a.n * units);
+  if (blockIdx.x == 0 && tid == 0) pl.first[a.n + 1] = per, pl.first[a.n + 2] = pad;
   const int64_t begin = blockIdx.x * per, end = min(first[a.n], begin + per);
   const float f = a.scale * LOG2E;
   const int key = lane & 15, kq = lane >> 4;  // of a score; of a key's dims
@@ -195,10 +245,10 @@ __global__ __launch_bounds__(256, split_per_cu(TYPE, HS, GT)) void k_paged_split
       }
       e = lo;
     }
-    const int cnt = count[e];
+    const int cnt = count[e], room = padded(cnt, pad);
     const int64_t rel = u - first[e];
-    const int hu = __builtin_amdgcn_readfirstlane((int)quotient(rel, cnt));
-    const int gi0 = __builtin_amdgcn_readfirstlane((int)(rel - (int64_t)hu * cnt));
+    const int hu = __builtin_amdgcn_readfirstlane((int)quotient(rel, room));
+    const int gi0 = __builtin_amdgcn_readfirstlane((int)(rel - (int64_t)hu * room));
     const int gi1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)cnt, gi0 + (end - u)));
     const int kvh = hu / pl.parts, h0 = (hu - kvh * pl.parts) * GT, heads = min(GT, group - h0);
     const int seq = __builtin_amdgcn_readfirstlane(sequence[e]);
@@ -526,7 +576,7 @@ __global__ __launch_bounds__(256, split_per_cu(TYPE, HS, GT)) void k_paged_split
       pl.ml[(slot * GT + tid) * 2] = stat[tid][0];
       pl.ml[(slot * GT + tid) * 2 + 1] = stat[tid][1];
     }
-    u += gi1 - gi0;
+    u += (gi1 == cnt ? room : gi1) - gi0;
   }
 }
 
@@ -541,11 +591,11 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a, SplitPlan pl, i
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int e = blockIdx.x / a.n_heads, h = blockIdx.x - e * a.n_heads;
   const int status = *kv.status, cnt = pl.count[e];
-  const int64_t total = pl.first[a.n], before = pl.first[e];
+  const int64_t before = pl.first[e], per = pl.first[a.n + 1];
+  const int pad = (int)pl.first[a.n + 2];
   if (status != KV_OK || cnt == 0) return;
   const int group = a.n_heads / kv.n_kv, kvh = h / group, hg = h - kvh * group;
-  const int64_t per = stretch_of(total, pl.wgs, a.n * kv.n_kv * pl.parts);
-  const int64_t ua = before + (int64_t)(kvh * pl.parts + hg / pl.gt) * cnt;
+  const int64_t ua = before + (int64_t)(kvh * pl.parts + hg / pl.gt) * padded(cnt, pad);
   const int w0 = (int)quotient(ua, per), w1 = (int)quotient(ua + cnt - 1, per);
   if (w0 == w1) return;
   const int n = w1 - w0 + 1, g = hg % pl.gt;
@@ -621,7 +671,7 @@ static size_t split_layout(const PagedArgs &a, const DevInfo &dev, char *base, S
     off += (bytes + 255) & ~size_t(255);
     return at;
   };
-  p->first = (int64_t *)add(8 * (size_t)(a.n + 1));
+  p->first = (int64_t *)add(8 * (size_t)(a.n + 3));
   p->count = (int32_t *)add(4 * (size_t)a.n);
   p->part = (float *)add(sizeof(float) * 2 * (size_t)p->wgs * p->gt * a.kv.hs);
   p->ml = (float *)add(sizeof(float) * 4 * (size_t)p->wgs * p->gt);
