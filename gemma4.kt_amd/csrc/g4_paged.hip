@@ -98,8 +98,6 @@ constexpr int segment_worth(int type, int hs) {
   return groups < 4 ? 4 : groups;
 }
 
-G4_DEV int padded(int count, int pad) { return pad == 1 ? count : (count + pad - 1) / pad * pad; }
-
 // A score whose products or sums the matrix cores could not form (an infinite key times
 // a part that is zero, a sum beyond fp32): the dot product as it is written.
 template <int TYPE>

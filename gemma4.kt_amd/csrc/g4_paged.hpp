@@ -59,6 +59,9 @@ G4_DEV int64_t quotient(int64_t a, int64_t b) {
   return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
+// count up to a multiple of pad
+G4_DEV int padded(int count, int pad) { return pad == 1 ? count : (count + pad - 1) / pad * pad; }
+
 // v + the value of lane ^ S; for S = 16 and 32 one swap gives both sides in every lane
 template <int S>
 G4_DEV float add_partner(float v, int lane) {

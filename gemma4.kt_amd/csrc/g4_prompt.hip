@@ -21,7 +21,7 @@
 //
 // The (kv head, query tile, key tile) units are cut into equal stretches, one per
 // persistent workgroup, whatever the lengths, windows and causal triangles are
-// (k_prompt_plan counts them); a query tile whose key tiles are spread over several
+// (k_prompt_plan counts them; few query tiles are cut so that no stretch has parts of two); a query tile whose key tiles are spread over several
 // stretches leaves (maximum, sum, O) of each in a slot, and k_paged_prompt_join adds them.
 // A row whose sums are not finite (an infinite or NaN key or value among those it meets,
 // maybe hidden from it) is computed again by k_paged_prompt_join, from the formula: a
@@ -38,13 +38,13 @@
 //     instructions, 60% of their cycles.  The transposed reads of values are 16% of the time
 //     (441 us for 4096 tokens, 371 with a tile's first operands used throughout)
 //   four chunks of 301 to 1100 rows behind up to 12001 tokens, window 4096, 16/4 heads of 128,
-//     F16    187 us: 388 TFLOP/s; 4.9 vector instructions to a matrix instruction (the
+//     F16    182 us: 399 TFLOP/s; 4.9 vector instructions to a matrix instruction (the
 //     weights of a row are the same work for a head of 128 as for one of 256).  Without any
 //     reads from LDS it would be 177 us
-//   8 sequences of 5 drafted tokens behind 1000 to 16384, 16/8 heads of 256, BF16    101 us,
-//     3.9 TB/s: one wave of eight has rows, and computes as long as a tile's 64 KB take
-//   1001 tokens in a window of 512, 8/2 heads of 256, F16    48 us: three key tiles a
-//     stretch, so mostly its start and end, and the two small kernels
+//   8 sequences of 5 drafted tokens behind 1000 to 16384, 16/8 heads of 256, BF16    92 us,
+//     4.3 TB/s: one wave of eight has rows, and computes as long as a tile's 64 KB take
+//   1001 tokens in a window of 512, 8/2 heads of 256, F16    44 us: five key tiles a
+//     stretch, so as much its start and end, and the two small kernels
 #include "g4_paged.hpp"
 
 namespace g4 {
@@ -63,7 +63,7 @@ struct PromptTile {
 
 struct PromptPlan {
   int32_t *n_tiles;   // query tiles of a kv head part
-  int64_t *total;     // their key tiles, and those of a stretch
+  int64_t *total;     // their key tiles, those of a stretch, and what a query tile's are padded to
   int32_t *start;     // [wgs][2] the query tile and the unit (kv head part) that a stretch begins in
   PromptTile *tiles;  // [cap]
   uint16_t *odd;      // [cap][units][bm / 16] rows whose sums are not finite, of tiles in one stretch
@@ -124,9 +124,10 @@ G4_DEV int last_not_above(F at, int n, int64_t x) {
 
 // One workgroup: the query tiles of every sequence in order, with their key tiles, and
 // the tile that each stretch begins in.  5.5 us, all of it latency: two loads that depend on
-// each other, two scans, a search in LDS.
+// each other, two or three scans, a search in LDS.
 __global__ __launch_bounds__(1024) void k_prompt_plan(PagedArgs a, PromptPlan pl) {
   __shared__ int tiles[1025], wsum[16], rows[1024], ends[1024], seqs[1024], lens[1024];
+  __shared__ int counts[1024];
   __shared__ int64_t wsum64[16], firsts[1024];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const int status = *a.kv.status;  // looked at once the rest is here too
@@ -144,19 +145,14 @@ __global__ __launch_bounds__(1024) void k_prompt_plan(PagedArgs a, PromptPlan pl
     if (tid == 0) *a.kv.status = KV_BAD_DATA;
     return;
   }
-  int x = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d, 64);
-    if (lane >= d) x += y;
-  }
+  int x = wave_scan(mine);
   if (lane == 63) wsum[wid] = x;
   __syncthreads();
   for (int w = 0; w < wid; ++w) x += wsum[w];
   tiles[tid + 1] = x;
   if (tid == 0) tiles[0] = 0;
   __syncthreads();
-  const int n_tiles = tiles[a.n];  // at most cap
+  const int n_tiles = tiles[a.n], units = a.kv.n_kv * pl.parts;  // at most cap tiles
   int64_t before = 0;
   for (int t0 = 0; t0 < n_tiles; t0 += 1024) {
     const int t = t0 + tid;
@@ -191,13 +187,47 @@ __global__ __launch_bounds__(1024) void k_prompt_plan(PagedArgs a, PromptPlan pl
     if (t < n_tiles) {
       it.first = mybase + s - it.count;
       pl.tiles[t] = it;
-      if (t0 == 0) firsts[t] = it.first;
+      if (t0 == 0) firsts[t] = it.first, counts[t] = it.count;
     }
     before += all;
     __syncthreads();
   }
-  const int64_t all = before * a.kv.n_kv * pl.parts, per = prompt_stretch(all, pl.wgs);
-  if (tid == 0) *pl.n_tiles = n_tiles, pl.total[0] = before, pl.total[1] = per;
+  int64_t per = prompt_stretch(before * units, pl.wgs);
+  int pad = 1;
+  if (per > 1 && n_tiles <= 1024 && n_tiles * units <= pl.wgs) {
+    // Stretches that end where query tiles do, if that makes them no longer than a second
+    // segment would (its queries, first key tile and result take as long as three key tiles):
+    // the shortest of four lengths with which every piece has a workgroup.  1001 tokens in a
+    // window of 512, 8/2 heads of 256, F16: 44.4 us, 49.2 with equal stretches; 8 sequences of
+    // 5 drafted tokens 92 and 101.
+    auto wave_total = [](int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); };
+    bool aligned = false;
+    for (int i = 3; i >= 0; --i) {
+      const uint32_t p = (int)min(per, (int64_t)1 << 26) + i;
+      int pieces = 0;
+      for (int r = lane; r < n_tiles; r += 64) pieces += min((counts[r] + p - 1) / p, 1u << 20);
+      if (wave_total(pieces) > pl.wgs / units) break;
+      pad = p, aligned = true;
+    }
+    if (aligned) {
+      per = pad;
+      const int mine = tid < n_tiles ? (int)((uint32_t)(counts[tid] + pad - 1) / (uint32_t)pad) : 0;
+      const int s = wave_scan(mine);
+      if (lane == 63) wsum[wid] = s;
+      __syncthreads();
+      int base = s - mine;
+      before = 0;
+      for (int w = 0; w < 16; ++w) {
+        if (w < wid) base += wsum[w];
+        before += wsum[w];
+      }
+      before *= pad;
+      if (tid < n_tiles) pl.tiles[tid].first = firsts[tid] = (int64_t)base * pad;
+      __syncthreads();
+    }
+  }
+  const int64_t all = before * units;
+  if (tid == 0) *pl.n_tiles = n_tiles, pl.total[0] = before, pl.total[1] = per, pl.total[2] = pad;
   if (before == 0) return;
   if (n_tiles > 1024) {
     __threadfence_block();  // the tiles, for the search
@@ -272,6 +302,7 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
   if (*kv.status != KV_OK) return;
   const int group = a.n_heads / kv.n_kv, units = kv.n_kv * pl.parts, n_tiles = *pl.n_tiles;
   const int64_t per_unit = pl.total[0], per = pl.total[1], total = per_unit * units;
+  const int pad = (int)pl.total[2];
 
   // Workgroups b, b + 8, ... run on one XCD: they take neighbouring stretches, so that
   // the key tiles of a kv head are read into few L2s.
@@ -654,7 +685,7 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
         if (g4 == 0 && row_ok) pl.ml[(slot * BM + r) * 2] = m, pl.ml[(slot * BM + r) * 2 + 1] = l;
       }
     }
-    u += j1 - j0;
+    u += (j1 == cnt ? padded(cnt, pad) : j1) - j0;
   }
 }
 
@@ -876,7 +907,7 @@ static size_t prompt_layout(const PagedArgs &a, const DevInfo &dev, char *base, 
   };
   const size_t cap = (size_t)p->cap, units = (size_t)a.kv.n_kv * p->parts;
   p->n_tiles = (int32_t *)add(4);
-  p->total = (int64_t *)add(16);
+  p->total = (int64_t *)add(24);
   p->start = (int32_t *)add(8 * (size_t)p->wgs);
   p->tiles = (PromptTile *)add(sizeof(PromptTile) * cap);
   p->odd = (uint16_t *)add(2 * cap * units * (p->bm / 16));
