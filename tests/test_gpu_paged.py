@@ -890,3 +890,35 @@ def test_two_graphs_share_a_context(g4, ctx):
     finally:
         torch.cuda.synchronize()
         c2.close()
+
+
+@pytest.mark.parametrize("typ,window,sinks", [("f16", 0, 0), ("bf16", 150, 5), ("f32", 0, 0)], ids=str)
+def test_more_heads_than_workgroups(g4, run, typ, window, sinks):
+    """Decode and prompts with more heads, or query tiles, than the chip takes at once: their
+    stretches cross from one to the next, and heads lie in up to three of them."""
+    announce("more heads than workgroups, %s" % typ)
+    kv, hs = 8, 64
+    g = gen(81)
+    lengths = [int(x) for x in torch.randint(1, 260, (75,), generator=g)] + [2500, 0, 1]
+    cache = filled(g4, run, 82, typ, 1, kv, hs, 16, lengths)
+    model = Model(cache)
+    order = [int(x) for x in torch.randperm(len(lengths), generator=g)]
+    q = normal(g, len(order), 16, hs).cuda()
+    out = torch.empty_like(q)
+    g4.paged_attention_dev(run, cache, 0, q, out, 16, i32(order), 0.12, window, sinks)
+    torch.cuda.synchronize()
+    rows = list(range(0, 78, 5)) + [order.index(75), order.index(76), order.index(77)]
+    check_rows(out, [(r, order[r], lengths[order[r]] - 1) for r in rows], model, 0, q, 0.12, window, sinks)
+    # 64 heads: 24 tokens to a query tile, 8 * (105 + 1 + 9) of them
+    p = normal(g, 2720, 64, hs).cuda()
+    out = torch.full_like(p, 7.0)
+    begin = [0, 2500, 2501, 2709]
+    seqs = [75, 77, 0]
+    g4.paged_prompt_dev(run, cache, 0, p, out, 64, i32(seqs), i32(begin), 2720, 0.12, window, sinks)
+    torch.cuda.synchronize()
+    places = [(r, seqs[i], lengths[seqs[i]] - (begin[i + 1] - begin[i]) + r - begin[i]) for i in range(3)
+              for r in range(begin[i], begin[i + 1]) if r % 173 == 0 or r in (1, 2499, 2500, 2501, 2708)]
+    check_rows(out, [x for x in places if x[2] >= 0], model, 0, p, 0.12, window, sinks)
+    for r, _, pos in places:
+        assert pos >= 0 or bool((out[r] == 0).all())
+    assert bool((out[2709:] == 7.0).all())
