@@ -165,18 +165,18 @@ __global__ __launch_bounds__(256, split_per_cu(TYPE, HS, GT)) void k_paged_split
       // (Sums in 32 bits: of counts cut to 2^21 groups, for the lengths to try only.)
       // 24 rows in a window of 1024, 8/1 heads of 512, BF16: 27.2 us, 34.4 with equal stretches;
       // 30 of up to 3000 in a window of 512, 8/2 of 128, F16: 17.4 and 21.5; one row whose heads
-      // fill equal stretches anyway pays 0.3 us for the choice.
+      // fill equal stretches anyway takes as long.
       __syncthreads();
       auto wave_total = [](int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); };
       int all = 0;
       for (int r = lane; r < a.n; r += 64) all += min(count[r], 1 << 21);
       const int least = (int)stretch_of((int64_t)wave_total(all) * units, gridDim.x, a.n * units);
-      for (int i = 2; i >= 0; --i) {
+      for (int i = 0; i < 3 && !aligned; ++i) {
         const uint32_t p = least + i * (segment_worth(TYPE, HS) / 2);
         int pieces = 0;
         for (int r = lane; r < a.n; r += 64) pieces += min((count[r] + p - 1) / p, 1u << 20);
-        if (wave_total(pieces) > (int)gridDim.x / units) break;
-        pad = p, aligned = true;
+        aligned = wave_total(pieces) <= (int)gridDim.x / units;
+        if (aligned) pad = p;
       }
     }
     // first: sums of 64 bits, or of the heads' pieces, of which there are few

@@ -198,16 +198,16 @@ __global__ __launch_bounds__(1024) void k_prompt_plan(PagedArgs a, PromptPlan pl
     // Stretches that end where query tiles do, if that makes them no longer than a second
     // segment would (its queries, first key tile and result take as long as three key tiles):
     // the shortest of four lengths with which every piece has a workgroup.  1001 tokens in a
-    // window of 512, 8/2 heads of 256, F16: 44.4 us, 49.2 with equal stretches; 8 sequences of
+    // window of 512, 8/2 heads of 256, F16: 42 to 44 us, 49 with equal stretches; 8 sequences of
     // 5 drafted tokens 92 and 101.
     auto wave_total = [](int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); };
     bool aligned = false;
-    for (int i = 3; i >= 0; --i) {
+    for (int i = 0; i < 4 && !aligned; ++i) {
       const uint32_t p = (int)min(per, (int64_t)1 << 26) + i;
       int pieces = 0;
       for (int r = lane; r < n_tiles; r += 64) pieces += min((counts[r] + p - 1) / p, 1u << 20);
-      if (wave_total(pieces) > pl.wgs / units) break;
-      pad = p, aligned = true;
+      aligned = wave_total(pieces) <= pl.wgs / units;
+      if (aligned) pad = p;
     }
     if (aligned) {
       per = pad;
