@@ -4,7 +4,7 @@
 // Every row is a token of a sequence and a query head; it sees what g4_paged.hip says,
 // causally.  A query tile is up to BM rows of one sequence that share a kv head: its
 // consecutive tokens times the heads of that kv head.  Keys and values come in tiles of
-// KT tokens through LDS (two buffers, loaded straight to LDS by half of the waves while
+// KT tokens through LDS (two buffers, loaded straight to LDS by four of the waves while
 // the other is worked on) and are used by all waves; a wave has 16 rows.
 //
 // Both products are on the matrix cores, transposed, so that a lane stays with one row
@@ -21,9 +21,9 @@
 //
 // The (kv head, query tile, key tile) units are cut into equal stretches, one per
 // persistent workgroup, whatever the lengths, windows and causal triangles are
-// (k_prompt_plan counts them; few query tiles are cut so that no stretch has parts of two); a query tile whose key tiles are spread over several
-// stretches leaves (maximum, sum, O) of each in a slot, and k_paged_prompt_join adds them.
-// A row whose sums are not finite (an infinite or NaN key or value among those it meets,
+// (k_prompt_plan counts them; few query tiles are cut so that no stretch has parts of
+// two).  A query tile whose key tiles are spread over several stretches leaves (maximum,
+// sum, O) of each in a slot, and k_paged_prompt_join adds them.  A row whose sums are not finite (an infinite or NaN key or value among those it meets,
 // maybe hidden from it) is computed again by k_paged_prompt_join, from the formula: a
 // prompt of nothing but NaN takes 25 times as long as any other.
 //
@@ -39,8 +39,8 @@
 //     (441 us for 4096 tokens, 371 with a tile's first operands used throughout)
 //   four chunks of 301 to 1100 rows behind up to 12001 tokens, window 4096, 16/4 heads of 128,
 //     F16    182 us: 399 TFLOP/s; 4.9 vector instructions to a matrix instruction (the
-//     weights of a row are the same work for a head of 128 as for one of 256).  Without any
-//     reads from LDS it would be 177 us
+//     weights of a row are the same work for a head of 128 as for one of 256).  Reads from
+//     LDS are 6% of it (188 us on one card, 177 without any)
 //   8 sequences of 5 drafted tokens behind 1000 to 16384, 16/8 heads of 256, BF16    92 us,
 //     4.3 TB/s: one wave of eight has rows, and computes as long as a tile's 64 KB take
 //   1001 tokens in a window of 512, 8/2 heads of 256, F16    44 us: five key tiles a
@@ -50,7 +50,8 @@
 namespace g4 {
 
 // A query tile: rows row .. row + toks - 1 of the call, the first at position `base`, of a
-// sequence with `len` tokens; `count` key tiles, `first` of them before its own.
+// sequence with `len` tokens; `count` key tiles, `first` (with those the others are padded
+// to) before its own.
 struct PromptTile {
   int32_t row;
   int32_t toks;
@@ -637,9 +638,9 @@ __global__ __launch_bounds__(64 * prompt_waves(HS), prompt_waves(HS) / 4) void k
       sign = -sign;
     };
 
-    // The loads of a tile's successor take their waves a while to issue.  The other wave
-    // of each of their SIMDs begins with the tile at once and so stays ahead: one has the
-    // matrix cores while the other forms weights.
+    // The loads of a tile's successor take their waves a while to issue.  The other waves
+    // of their SIMDs begin with the tile at once and so stay ahead: one has the matrix
+    // cores while another forms weights.
     if (loader >= 0) next_page = page_at(j0);
     tile_barrier();  // the last segment's tiles are done with
     if (loader >= 0) issue(j0);
