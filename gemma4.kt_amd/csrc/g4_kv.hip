@@ -292,10 +292,10 @@ __global__ __launch_bounds__(KV_RES) void k_kv_resolve(KvArgs kv, KvMove m, Plan
 // (lists, lengths, table, refs).  Sums by lane permutes and two counts a barrier took it
 // from 6.5 us.
 __global__ __launch_bounds__(KV_T) void k_kv_plan(KvArgs kv, KvMove m, Plan p) {
-  __shared__ int mark[KV_MAX_SEQS], ws[2 * KV_T / 64];
+  __shared__ int mark[KV_MAX_SEQS], taken[KV_MAX_SEQS], ws[2 * KV_T / 64];  // taken: full pages that an entry shares
   const int tid = threadIdx.x, status = *kv.status;
   const int free4 = four_free(kv, 0);  // on its way while the lists are read
-  mark[tid] = 0;
+  mark[tid] = taken[tid] = 0;
   bool bad = false;
   for (int i = tid; i < p.n_bad; i += KV_T) bad |= p.bad[i] != 0;
   __syncthreads();
@@ -303,9 +303,11 @@ __global__ __launch_bounds__(KV_T) void k_kv_plan(KvArgs kv, KvMove m, Plan p) {
     if (tid == 0) *p.ok = 0;
     return;
   }
-  int prefix = 0, shared = 0, length = 0, need = 0, copies = 0, src_page = -1;
+  int src = 0, prefix = 0, shared = 0, length = 0, need = 0, copies = 0, src_page = -1;
+  bool stays = false;
   if (tid < m.n) {
-    const int src = m.src[tid], dst = m.dst[tid];
+    src = m.src[tid];
+    const int dst = m.dst[tid];
     bool off = !in_range(src, kv.max_seqs) || !in_range(dst, kv.max_seqs);
     if (!off) {
       off = atomicAdd(&mark[dst], 1) > 0;
@@ -322,14 +324,12 @@ __global__ __launch_bounds__(KV_T) void k_kv_plan(KvArgs kv, KvMove m, Plan p) {
       if (!off) {
         length = prefix + listed;
         shared = prefix >> kv.shift;
+        atomicMax(&taken[src], shared);
         if (prefix & (kv.page - 1)) {
           src_page = kv.table[(int64_t)src * kv.max_pages + shared];
           off = !in_range(src_page, kv.n_pages);
-          // a sequence that stays where it is keeps its last page if no other holds it
-          if (!off && src == dst && listed == 0 && kv.refs[src_page] == 1) ++shared;
+          stays = !off && src == dst && listed == 0 && kv.refs[src_page] == 1;
         }
-        need = max(0, ((length + kv.page - 1) >> kv.shift) - shared);
-        copies = max(0, length - (shared << kv.shift));
       }
     }
     bad |= off;
@@ -337,6 +337,14 @@ __global__ __launch_bounds__(KV_T) void k_kv_plan(KvArgs kv, KvMove m, Plan p) {
   if (__syncthreads_or(bad)) {
     if (tid == 0) *kv.status = KV_BAD_DATA, *p.ok = 0;
     return;
+  }
+  if (tid < m.n) {
+    // A sequence that stays where it is keeps its last page if no other holds it, before the
+    // call or after it: a longer continuation takes the page over as a full one, and its
+    // tokens behind this prefix with it.
+    if (stays && taken[src] <= shared) ++shared;
+    need = max(0, ((length + kv.page - 1) >> kv.shift) - shared);
+    copies = max(0, length - (shared << kv.shift));
   }
   // The lists of kept tokens follow each other, so the copies are at most n_keep + n * page,
   // which the host has checked, and the pages fewer.

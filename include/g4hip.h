@@ -338,7 +338,8 @@ int g4_kv_extend_dev(g4_ctx *ctx, const g4_kv *kv, int32_t n, const int32_t *d_s
  * one, in all layers, and what d_dst[i] held is given back.  A sequence may be the
  * source of several and itself be replaced (beams that are reordered): all read the
  * state before the call.  d_src[i] = d_dst[i] shortens, and copies nothing where the last
- * page is its own.  Fresh pages are free before the call.  Two launches. */
+ * page is its own and no other entry shares it.  Fresh pages are free before the call.
+ * Two launches. */
 int g4_kv_fork_dev(g4_ctx *ctx, const g4_kv *kv, int32_t n, const int32_t *d_src, const int32_t *d_dst,
                    const int32_t *d_lengths);
 /* Sequence d_dst[i] becomes the first d_prefix[i] tokens of d_src[i] (d_prefix NULL: none),
