@@ -568,16 +568,91 @@ G4_DEV void rotate(bool turn, bool pairs, const float (&c)[N], const float (&s)[
   }
 }
 
+// A write is all or nothing.  Its rows are looked at through LDS lists of its entries:
+struct WriteList {
+  int mark[KV_MAX_SEQS];       // times that a sequence is named
+  int first[KV_MAX_SEQS + 1];  // first row of an entry
+  int len[KV_MAX_SEQS];
+  int seq[KV_MAX_SEQS];
+};
+
+G4_DEV int page_of(const KvArgs &kv, int seq, int len, int pos) {  // -1: out of range
+  return in_range(pos, len) ? kv.table[(int64_t)seq * kv.max_pages + (pos >> kv.shift)] : -1;
+}
+
+// A page that can be written: it is there, and no other sequence holds it.
+G4_DEV bool own_page(const KvArgs &kv, int page) { return in_range(page, kv.n_pages) && kv.refs[page] == 1; }
+
+// The entries read into the list by T threads.  True: the thread met one that does not rise.
+template <int T>
+G4_DEV bool read_write_list(const KvArgs &kv, const KvWrite &w, WriteList &l) {
+  bool bad = false;
+  for (int i = threadIdx.x; i < kv.max_seqs; i += T) l.mark[i] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < w.n; i += T) {
+    const int seq = w.seqs[i];
+    int from = i, to = i + 1;
+    if (w.row_begin) {
+      from = w.row_begin[i], to = w.row_begin[i + 1];
+      bad |= from < 0 || to < from || to > w.n_rows;
+    }
+    l.first[i] = from;
+    if (i + 1 == w.n) l.first[w.n] = to;
+    l.seq[i] = seq, l.len[i] = safe_length(kv, seq);
+    if (in_range(seq, kv.max_seqs)) atomicAdd(&l.mark[seq], 1);
+  }
+  return bad;
+}
+
+// Then the pages: those of the first and last row of each entry, and those between, each of
+// which holds a row whose number is a multiple of a page's tokens.  `meanwhile` is done
+// while the thread's first pages are on their way.
+template <int T, class F>
+G4_DEV bool check_write_list(const KvArgs &kv, const KvWrite &w, const WriteList &l, F meanwhile) {
+  bool bad = false;
+  auto ends = [&](int i, int &a, int &b) {  // false: an entry without rows needs no page
+    const int rows = i < w.n ? l.first[i + 1] - l.first[i] : 0;
+    if (rows == 0) return false;
+    a = page_of(kv, l.seq[i], l.len[i], l.len[i] - rows);
+    b = rows > 1 ? page_of(kv, l.seq[i], l.len[i], l.len[i] - 1) : a;
+    return true;
+  };
+  auto check = [&](int i, int a, int b) { bad |= !own_page(kv, a) || (b != a && !own_page(kv, b)) || l.mark[l.seq[i]] > 1; };
+  int a, b;
+  const bool some = ends(threadIdx.x, a, b);
+  meanwhile();
+  if (some) check(threadIdx.x, a, b);
+  for (int i = threadIdx.x + T; i < w.n; i += T)
+    if (ends(i, a, b)) check(i, a, b);
+  if (w.row_begin)
+    for (int64_t row = (int64_t)threadIdx.x << kv.shift; row < l.first[w.n]; row += (int64_t)T << kv.shift) {
+      if (row < l.first[0]) continue;
+      const int e = find_entry(l.first, w.n, (int)row);
+      bad |= !own_page(kv, page_of(kv, l.seq[e], l.len[e], l.len[e] - l.first[e + 1] + (int)row));
+    }
+  return bad;
+}
+
+__global__ __launch_bounds__(KV_T) void k_kv_write_check(KvArgs kv, KvWrite w) {
+  __shared__ WriteList l;
+  if (*kv.status != KV_OK) return;
+  bool bad = __syncthreads_or(read_write_list<KV_T>(kv, w, l));
+  if (!bad) bad = __syncthreads_or(check_write_list<KV_T>(kv, w, l, [] {}));
+  if (bad && threadIdx.x == 0) *kv.status = KV_BAD_DATA;
+}
+
 // A workgroup turns a stretch of the heads of one row (blockIdx.x; blockIdx.y of
 // gridDim.y stretches): thread (slot, u) takes unit u of every slots-th head and so
 // forms its cosines once.  Heads 0 .. n_heads - 1 are q, then n_kv of k, then n_kv of v.
-// Bound by memory for prompts (8000 rows of 32/4 heads of 128, F16: 64 us, 4.8 TB/s of the
-// 5.1 that a copy reaches) and by latency for single rows (32 of them 7.5 us: the row's
-// sequence, its length, page and owner are four loads that wait for each other, and its
-// first head comes meanwhile).
-template <int TYPE, int N>
+// CHECK: every workgroup looks at the whole call before it writes.  All find the same, so a
+// call that cannot be done writes nothing, whichever of them sets *status first; otherwise
+// k_kv_write_check has looked.
+// Bound by memory for prompts and by latency for single rows: 7900 rows of 32/4 heads of 128,
+// F16: 60 us, 5.1 TB/s, as a copy; 32 rows of 16/8 heads of 256, BF16: 5.8 us, 1 us of it the
+// look at the whole call.
+template <int TYPE, int N, bool CHECK>
 __global__ __launch_bounds__(256) void k_kv_write(KvArgs kv, RopeArgs r, KvWrite w) {
-  __shared__ int begin[KV_MAX_SEQS];
+  __shared__ WriteList l;
   const int row = blockIdx.x, tid = threadIdx.x;
   const int status = *kv.status;
   const int units = kv.hs / (2 * N), slots = 256 / units, slot = tid / units, u = tid % units;
@@ -597,40 +672,43 @@ __global__ __launch_bounds__(256) void k_kv_write(KvArgs kv, RopeArgs r, KvWrite
     load_floats<N>(from + b, y);
   };
   if (h0 + slot < h1) load(h0 + slot);  // on its way while the row's place is looked up
-  if (status != KV_OK) return;
-  int e = row, rows = 1, at = 0;
-  bool bad = false;
-  if (w.row_begin) {
-    for (int i = tid; i < w.n; i += 256) {
-      const int from = w.row_begin[i], to = w.row_begin[i + 1];
-      bad |= from < 0 || to < from || to > w.n_rows;
-      begin[i] = from;
-    }
-    const int last = w.row_begin[w.n];
-    if (__syncthreads_or(bad)) {
+  if constexpr (CHECK) {
+    // A wave may see what another workgroup of this launch has set: all waves decide together.
+    if (__syncthreads_or(read_write_list<256>(kv, w, l) || status != KV_OK)) {
       if (tid == 0) atomicCAS(kv.status, KV_OK, KV_BAD_DATA);
       return;
     }
-    if (row < begin[0] || row >= last) return;  // behind the last sequence: left as it is
-    e = find_entry(begin, w.n, row);
-    rows = w.row_begin[e + 1] - begin[e];
-    at = row - begin[e];
+  } else {
+    if (status != KV_OK) return;  // nobody sets it in this launch
+    if (w.row_begin) {
+      for (int i = tid; i <= w.n; i += 256) l.first[i] = w.row_begin[i];
+      __syncthreads();
+    }
   }
-  const int seq = w.seqs[e], len = safe_length(kv, seq);
-  for (int i = tid; i < w.n; i += 256) bad |= i != e && w.seqs[i] == seq;  // two rows for one place
-  const int pos = len - rows + at;
-  int page = -1;
-  if (pos >= 0 && pos < len) page = kv.table[(int64_t)seq * kv.max_pages + (pos >> kv.shift)];
+  int e = row, to_end = 1;  // the row's entry, and how far before its end the row stands
+  bool mine = true;         // rows of no sequence are left as they are
+  if (w.row_begin) {
+    mine = row >= l.first[0] && row < l.first[w.n];
+    e = find_entry(l.first, w.n, row);
+    to_end = l.first[e + 1] - row;
+  }
+  const int seq = CHECK ? l.seq[e] : w.seqs[e], len = CHECK ? l.len[e] : safe_length(kv, seq);
+  const int pos = len - to_end, page = mine ? page_of(kv, seq, len, pos) : -1;
   float c[N], s[N];
-  if (turn && h0 + slot < min(h1, w.n_heads + kv.n_kv))
+  auto turns = [&] {
+    if (turn && h0 + slot < min(h1, w.n_heads + kv.n_kv))
 #pragma unroll
-    for (int i = 0; i < N; ++i) turn_of((double)pos, r.freqs[u * N + i], r.gain, c[i], s[i]);
-  // the page is there, and no other sequence holds it
-  bad |= !in_range(page, kv.n_pages) || kv.refs[page] != 1;
-  if (__syncthreads_or(bad)) {
-    if (tid == 0) atomicCAS(kv.status, KV_OK, KV_BAD_DATA);
-    return;
+      for (int i = 0; i < N; ++i) turn_of((double)pos, r.freqs[u * N + i], r.gain, c[i], s[i]);
+  };
+  if constexpr (CHECK) {
+    if (__syncthreads_or(check_write_list<256>(kv, w, l, turns))) {
+      if (tid == 0) atomicCAS(kv.status, KV_OK, KV_BAD_DATA);
+      return;
+    }
+  } else {
+    turns();
   }
+  if (!in_range(page, kv.n_pages)) return;
   for (int h = h0 + slot; h < h1;) {
     const bool is_q = h < w.n_heads, is_k = !is_q && h < w.n_heads + kv.n_kv;
     rotate<N>(turn && (is_q || is_k), r.pairs, c, s, x, y);
@@ -706,21 +784,36 @@ hipError_t launch_rope(const RopeArgs &r, const float *x, float *out, int32_t n_
   return hipGetLastError();
 }
 
-template <int TYPE>
+template <int TYPE, bool CHECK>
 static void launch_write(const KvArgs &kv, const RopeArgs &r, const KvWrite &w, hipStream_t s) {
   const int heads = w.n_heads + 2 * kv.n_kv;
   if (r.rot % 8 == 0 && aligned16(w.q) && aligned16(w.q_out) && aligned16(w.k) && aligned16(w.v))
-    hipLaunchKernelGGL((k_kv_write<TYPE, 4>), dim3(w.n_rows, row_split(w.n_rows, heads, 256 / (kv.hs / 8))), dim3(256),
-                       0, s, kv, r, w);
+    hipLaunchKernelGGL((k_kv_write<TYPE, 4, CHECK>), dim3(w.n_rows, row_split(w.n_rows, heads, 256 / (kv.hs / 8))),
+                       dim3(256), 0, s, kv, r, w);
   else
-    hipLaunchKernelGGL((k_kv_write<TYPE, 1>), dim3(w.n_rows, row_split(w.n_rows, heads, 256 / (kv.hs / 2))), dim3(256),
-                       0, s, kv, r, w);
+    hipLaunchKernelGGL((k_kv_write<TYPE, 1, CHECK>), dim3(w.n_rows, row_split(w.n_rows, heads, 256 / (kv.hs / 2))),
+                       dim3(256), 0, s, kv, r, w);
+}
+
+template <int TYPE>
+static void launch_write(const KvArgs &kv, const RopeArgs &r, const KvWrite &w, bool check, hipStream_t s) {
+  if (check) launch_write<TYPE, true>(kv, r, w, s);
+  else launch_write<TYPE, false>(kv, r, w, s);
 }
 
 hipError_t launch_kv_write(const KvArgs &kv, const RopeArgs &r, const KvWrite &w, hipStream_t s) {
-  if (kv.type == T_F32) launch_write<T_F32>(kv, r, w, s);
-  else if (kv.type == T_F16) launch_write<T_F16>(kv, r, w, s);
-  else launch_write<T_BF16>(kv, r, w, s);
+  // Few rows are looked at by every workgroup, many by one before them: 32 rows take 5.8 and
+  // 7.2 us, 512 10.7 and 11.5, 2000 of one sequence 17.7 and 18.7, 2560 of 64 22.1 and 22.4, 3000
+  // of three 23.9 and 23.8, 8000 of one 66.9 and 57.6.
+  const bool check = w.n_rows <= 2048;
+  if (!check) {
+    hipLaunchKernelGGL(k_kv_write_check, dim3(1), dim3(KV_T), 0, s, kv, w);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if (kv.type == T_F32) launch_write<T_F32>(kv, r, w, check, s);
+  else if (kv.type == T_F16) launch_write<T_F16>(kv, r, w, check, s);
+  else launch_write<T_BF16>(kv, r, w, check, s);
   return hipGetLastError();
 }
 

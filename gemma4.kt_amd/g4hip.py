@@ -852,7 +852,8 @@ def rope_dev(ctx: Context, rope: Rope, x, out, n_rows: int, n_heads: int, head_s
 def kv_rope_write_dev(ctx: Context, cache: KvCache, layer: int, q, q_out, k, v, n_heads: int, rope: Optional[Rope],
                       seqs, row_begin, n_rows: int) -> None:
     """Turn q to q_out (both None: no queries) and k, and write k and v as the last rows
-    of their sequences in a layer (row_begin None: one row per sequence)."""
+    of their sequences in a layer (row_begin None: one row per sequence): all rows, or
+    none and kv_status says so."""
     at, n = _dev_list(ctx, seqs, "seqs")
     size = n_rows * n_heads * cache.head_size
     kv_size = n_rows * cache.n_kv_heads * cache.head_size

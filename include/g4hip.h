@@ -396,9 +396,9 @@ int g4_rope_dev(g4_ctx *ctx, const g4_rope *rope, const float *d_x, float *d_out
  * queries), d_k [n_rows][n_kv_heads][head_size] is turned and d_v taken as it is, and
  * both are written to the sequence's pages, rounded to nearest (F16 overflows to
  * infinity).  rope NULL: nothing is turned, and d_q is NULL.  Rows of no sequence
- * are left as they are.  A row whose page is not there or is shared, or whose sequence is
- * named twice, is not written, and *status is set; no row is if d_row_begin does not
- * rise.  One launch. */
+ * are left as they are.  All or nothing: if a row's page is not there or is shared, a sequence
+ * with rows is named twice, or d_row_begin does not rise, nothing is written, to d_q_out
+ * neither, and *status is set.  One launch, two for more than 2048 rows. */
 int g4_kv_rope_write_dev(g4_ctx *ctx, const g4_kv *kv, int32_t layer, const g4_rope *rope, const float *d_q,
                          float *d_q_out, const float *d_k, const float *d_v, int32_t n_heads, int32_t n,
                          const int32_t *d_seqs, const int32_t *d_row_begin, int32_t n_rows);
