@@ -738,14 +738,20 @@ class KvCache:
     @staticmethod
     def create(ctx: Context, n_layers: int, n_kv_heads: int, head_size: int, page_tokens: int, n_pages: int,
                max_seqs: int, max_pages: int, dtype=None) -> "KvCache":
-        """An empty cache in new tensors (dtype: a torch type, bfloat16 by default)."""
+        """An empty cache in new tensors (dtype: a torch type, bfloat16 by default).  They are
+        filled on torch's current stream, which is waited for: calls of `ctx` on any stream
+        may follow.  (In a capture the fills are recorded, and the caller orders what follows.)"""
         import torch
         dev = torch.device("cuda", ctx.ordinal)
         shape = (n_layers, n_pages, n_kv_heads, page_tokens, head_size)
         k, v = (torch.zeros(shape, dtype=dtype or torch.bfloat16, device=dev) for _ in range(2))
         i32 = dict(dtype=torch.int32, device=dev)
-        return KvCache(k, v, torch.full((max_seqs, max_pages), -1, **i32), torch.zeros(max_seqs, **i32),
-                       torch.zeros(n_pages, **i32), torch.zeros(1, **i32))
+        cache = KvCache(k, v, torch.full((max_seqs, max_pages), -1, **i32), torch.zeros(max_seqs, **i32),
+                        torch.zeros(n_pages, **i32), torch.zeros(1, **i32))
+        with torch.cuda.device(dev):
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream().synchronize()
+        return cache
 
     def on(self, ctx: Context) -> int:
         """Address of the description, for a call of `ctx`."""
