@@ -26,7 +26,8 @@ namespace g4 {
 //
 // A wave takes NG groups at a time.  Scores come from the matrix cores: A = the query
 // heads, B = 16 keys as they lie in memory.  A head is four rows of A: for a 16-bit
-// cache the query's three 16-bit parts, which add up to it exactly, for F32 the query
+// cache the query's three 16-bit parts, which add up to it (BF16 exactly, F16 to 2^-39 of
+// its largest element), for F32 the query
 // itself; the products are then exact (F32: rounded once), and a lane's sum over its
 // four rows of C is the score of (head lane / 16, key lane % 16).  The queries carry
 // scale * log2(e) (split_scale keeps their parts in range).  Values are weighted by the

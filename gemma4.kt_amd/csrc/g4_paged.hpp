@@ -119,7 +119,7 @@ struct Mfma<T_BF16> {
 
 // Two fp32 values' next 16-bit parts, in one word; the values become the remainders.
 // BF16 truncates: three parts hold the 24 bits of a finite value.  F16 rounds to
-// nearest, 11 bits and a sign a part, of values below 2 in size.
+// nearest, 11 bits and a sign a part, on steps of 2^-24 at least.
 template <int TYPE>
 G4_DEV uint32_t take_part(float &x, float &y) {
   if constexpr (TYPE == T_BF16) {
@@ -136,15 +136,17 @@ G4_DEV uint32_t take_part(float &x, float &y) {
 }
 
 // The power of two that a query of this size (its largest element's) is multiplied by
-// before it is split, and its inverse.  F16: to [1, 2), so that its parts are neither
-// subnormal nor too large; an F16 key is at most 65504, so sums stay finite.  BF16: only
-// queries so small that their parts would be subnormal.  1 where nothing is split.
+// before it is split, and its inverse.  F16: to [2^14, 2^15), the highest that no part
+// overflows, since parts stand on steps of 2^-24: what they leave out of an element is at
+// most 2^-39 of the largest one (2^-25 with that at 1), or 2^-22 of itself with two parts, none with
+// three.  An F16 key is at most 65504, so sums stay below 2^40.  BF16: only queries so
+// small that their parts would be subnormal.  1 where nothing is split.
 template <int TYPE>
 G4_DEV void split_scale(float size, float &to, float &back) {
   to = back = 1.f;
   if constexpr (TYPE == T_F16) {
-    const uint32_t e = __float_as_uint(size) >> 23 & 255;
-    if (e > 0 && e < 254) to = __uint_as_float((254u - e) << 23), back = __uint_as_float(e << 23);
+    const uint32_t e = max(__float_as_uint(size) >> 23 & 255, 15u);  // the inverse stays normal
+    to = __uint_as_float((268u - e) << 23), back = __uint_as_float((e - 14u) << 23);
   } else if constexpr (TYPE == T_BF16) {
     if (size < 0x1p-80f) to = 0x1p40f, back = 0x1p-40f;
   }

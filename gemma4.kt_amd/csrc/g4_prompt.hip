@@ -14,7 +14,8 @@
 //                 are the weights it needs, since the keys of a product may come in any
 //                 order as long as A and B agree
 // For BF16 the queries and the weights are three bf16 parts each, exact; for F16 two
-// f16 parts (22 bits) of values scaled by a power of two; an F32 cache takes the fp32
+// f16 parts (22 bits, and 2^-39 of a query's largest element) of values scaled by a power of
+// two, since a third part would add half to the matrix work; an F32 cache takes the fp32
 // products.  The running maximum and sum are fp32.  The matrix cores round every sum
 // down, so each tile's O^T is summed on its own, added in fp32, and every second tile
 // is computed with -P and subtracted: those errors then cancel instead of adding up.

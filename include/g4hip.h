@@ -410,15 +410,17 @@ int g4_kv_rope_write_dev(g4_ctx *ctx, const g4_kv *kv, int32_t layer, const g4_r
  *   out = sum_t exp(s_t - max) V[t] / sum_t exp(s_t - max)
  * over the tokens t <= p that it sees: all (window = 0), or t > p - window and the
  * first `sinks`.  A row that sees nothing (an empty sequence, pages given back, scores
- * that are all -infinity) is zeros.  fp32 products and sums.  d_q and d_out are 16-byte
+ * that are all -infinity) is zeros.  fp32 products and sums; over an F16 cache an element
+ * of a query is taken to 2^-39 of the largest of its head.  d_q and d_out are 16-byte
  * aligned and do not overlap.  Two launches. */
 int g4_paged_attention_dev(g4_ctx *ctx, const g4_kv *kv, int32_t layer, const float *d_q, float *d_out,
                            int32_t n_heads, int32_t n, const int32_t *d_seqs, float scale, int32_t window,
                            int32_t sinks);
 /* The same for several tokens per sequence (prompts, their chunks, drafted tokens): the
  * rows of each sequence as in g4_kv_rope_write_dev, each at its own position and seeing
- * no later one.  Rows of no sequence are left as they are; if d_row_begin does not rise,
- * all are, and *status is set.  Three launches. */
+ * no later one.  Over an F16 cache queries and weights are taken to 22 bits (2^-22 of each,
+ * and 2^-39 of the largest element of a query's head).  Rows of no sequence are left as they
+ * are; if d_row_begin does not rise, all are, and *status is set.  Three launches. */
 int g4_paged_prompt_dev(g4_ctx *ctx, const g4_kv *kv, int32_t layer, const float *d_q, float *d_out, int32_t n_heads,
                         int32_t n, const int32_t *d_seqs, const int32_t *d_row_begin, int32_t n_rows, float scale,
                         int32_t window, int32_t sinks);
