@@ -103,3 +103,54 @@ def test_subnormal_keys_and_values(g4, run, hs):  # noqa: F811
         for h in range(heads):
             o, size, a = exact(q[r, h], k[:, 0], v[:, 0], hs ** -0.5)
             assert bool(((out[r, h] - o).abs() <= bar("f16", hs, size, a)).all())
+
+
+def causal(q, k, v, first, scale):
+    """Rows of one head at positions first, first + 1 .. over k, v [tokens, head size] in 64 bits."""
+    s = (q.double() @ k.T) * scale
+    t = torch.arange(len(k), device=k.device)
+    s = s.masked_fill(t > first + torch.arange(len(q), device=k.device)[:, None], -float("inf"))
+    return torch.softmax(s, 1) @ v
+
+
+def cut(x, bits):
+    """fp32 values without all but their highest `bits` bits."""
+    return (x.view(torch.int32) & -(1 << (24 - bits))).view(torch.float32)
+
+
+@pytest.mark.parametrize("length", [150, 2500])
+@pytest.mark.parametrize("typ,parts", [("bf16", 16), ("f16", 11), ("f32", 16)])
+def test_errors_beside_the_largest_value(g4, run, typ, parts, length):  # noqa: F811
+    """|out - exact| <= 3e-6 max |v| for queries and keys of ordinary size.  A score of up to
+    8 (in powers of two) passes 12 matrix instructions of BF16 for 128 elements, 8 of F16 or 32
+    of F32, of which each leaves out 2^-24 of it on average: 32 * 2^-24 * 8 ln 2 = 1.1e-5 of a
+    weight at most.  A result is a mean of values with those weights, and what is common to
+    them cancels: below 1.1e-5 of a mean |v| of 0.8, where the largest |v| is above 4.
+    Queries with only `parts` bits, one 16-bit part fewer, err by more: that is checked here too, with
+    the formula."""
+    announce("errors of %s over %d tokens" % (typ, length))
+    hs, heads, kv = 128, 4, 2
+    cache = filled(g4, run, 116, typ, 1, kv, hs, 32, [length, length])
+    q = normal(gen(117), length, heads, hs, scale=2.0).cuda()
+    one = normal(gen(118), 2, heads, hs, scale=2.0).cuda()
+    out, last = torch.empty_like(q), torch.empty_like(one)
+    scale = hs ** -0.5
+    g4.paged_prompt_dev(run, cache, 0, q, out, heads, i32([1]), i32([0, length]), length, scale)
+    g4.paged_attention_dev(run, cache, 0, one, last, heads, i32([0, 1]), scale)
+    torch.cuda.synchronize()
+    m = Model(cache)
+    worst = less = 0.0
+    for s in (0, 1):
+        k, v, _ = (t.cuda() if isinstance(t, torch.Tensor) else t for t in m.rows(0, s, length))
+        for h in range(heads):
+            kh, vh = k[:, h // 2].contiguous(), v[:, h // 2].contiguous()
+            bound = 3e-6 * float(vh.abs().max())
+            o = causal(one[s:s + 1, h], kh, vh, length - 1, scale)
+            worst = max(worst, float((last[s:s + 1, h].double() - o).abs().max()) / bound)
+            if s == 1:
+                o = causal(q[:, h], kh, vh, 0, scale)
+                worst = max(worst, float((out[:, h].double() - o).abs().max()) / bound)
+                fewer = causal(cut(q[:, h].contiguous(), parts), kh, vh, 0, scale)
+                less = max(less, float((fewer - o).abs().max()) / bound)
+    print("[error] %s %d: %.2f of the bar, %.2f with a part fewer" % (typ, length, worst, less))
+    assert worst <= 1 and less > 1
