@@ -278,7 +278,8 @@ _ctx = None
 
 
 def _context():
-    """The program's one context, with its own stream."""
+    """The program's one context, on torch's current stream: inputs, calls and what reads their results are in
+    order.  Torch's default stream has no handle that a context takes, so the program leaves it for another."""
     global _ctx
     if _ctx is None:
         package = os.path.join(_ROOT, "gemma4.kt_amd")
@@ -286,16 +287,21 @@ def _context():
             sys.path.insert(0, package)
         import g4hip
         _ctx = g4hip.Context(0)
+    before = torch.cuda.current_stream()
+    if before.cuda_stream == 0:
+        torch.cuda.set_stream(torch.cuda.Stream())
+        torch.cuda.current_stream().wait_stream(before)
+    _ctx.set_stream(torch.cuda.current_stream().cuda_stream)
     return _ctx
 
 
 def prepare(case, seed):
+    ctx = _context() if own else None
     s = _inputs(case, seed)
     s["case"] = case
     if case["kind"] in ("rope", "decode", "prompt"):
         s["out"] = torch.empty_like(s["q"])
     if own:
-        ctx = _context()
         import g4hip
         s["ctx"] = ctx
         s["cache"] = g4hip.KvCache(s["k"], s["v"], s["table"], s["lengths"], s["refs"], s["status"])
