@@ -132,3 +132,52 @@ def test_pages_in_the_middle_of_many_rows(g4, run):  # noqa: F811
         g4.kv_rope_write_dev(run, cache, 0, None, None, k, k, 0, None, i32([0]), i32([first, first + rows]), first + rows)
         g4.kv_status(run, cache)
         assert int((cache.k == 1).sum()) == rows * 8 and np.array_equal(Model(cache).table, before.table)
+
+
+@pytest.mark.parametrize("rows", [40, 1500])
+def test_a_captured_write_meets_a_row_without_a_place(g4, rows):
+    """Recorded once and replayed, with eager calls between: replays write while every row has a
+    place, nothing at all while one has none, and go on after the status is cleared."""
+    announce("a captured write of 2 x %d rows" % rows)
+    c2 = g4.Context(0)
+    try:
+        cache = g4.KvCache.create(c2, 1, 1, 64, 16, 400, 2, 200, torch.float32)
+        seqs, begin = i32([1, 0]), i32([0, rows, 2 * rows])
+        rope = g4.Rope.create(c2, 64)
+        q, k, v = (torch.zeros(2 * rows, m, 64, device="cuda") for m in (2, 1, 1))
+        out = torch.empty_like(q)
+        g4.kv_extend_dev(c2, cache, seqs, i32([rows + 7, rows]))
+        g4.kv_status(c2, cache)
+        torch.cuda.synchronize()
+        graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(graph, stream=stream):
+            c2.set_stream(stream.cuda_stream)
+            g4.kv_rope_write_dev(c2, cache, 0, q, out, k, v, 2, rope, seqs, begin, 2 * rows)
+        c2.set_stream(None)
+        g, page = gen(125), int(cache.table[0, rows // 32])
+        for i in range(6):
+            for t in (q, k, v):
+                t.copy_(normal(g, *t.shape))
+            out.fill_(float("nan"))
+            bad = i % 3 == 1
+            cache.refs[page] = 3 if bad else 1
+            before = Model(cache)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            if bad:
+                assert int(cache.status_word.cpu()) == 2 and bool(torch.isnan(out).all())
+                before.same_contents(cache)
+                with pytest.raises(g4.IndexOutOfBoundsException):
+                    g4.kv_status(c2, cache)
+                continue
+            wrote, mine = [t.clone() for t in (out, cache.k, cache.v)], torch.empty_like(out)
+            torch.cuda.synchronize()
+            g4.kv_rope_write_dev(c2, cache, 0, q, mine, k, v, 2, rope, seqs, begin, 2 * rows)
+            g4.kv_status(c2, cache)
+            assert not bool(torch.isnan(mine).any()) and torch.equal(mine, wrote[0])
+            assert torch.equal(cache.k, wrote[1]) and torch.equal(cache.v, wrote[2])
+            assert not torch.equal(before.v, cache.v.cpu())
+    finally:
+        torch.cuda.synchronize()
+        c2.close()
