@@ -129,7 +129,8 @@ __global__ __launch_bounds__(256) void k_kv_init(KvArgs kv) {
 }
 
 // lengths[seqs[i]] += counts[i], with the pages that takes.  The free pages are found
-// by counting refs, 4096 at a time: latency, as in k_kv_plan.
+// by counting refs, 4096 at a time: latency, as in k_kv_plan (4.2 us for 32 sequences that grow
+// by a token, 4.7 for 1024).
 __global__ __launch_bounds__(KV_T) void k_kv_extend(KvArgs kv, int n, const int32_t *seqs, const int32_t *counts) {
   __shared__ int mark[KV_MAX_SEQS], first[KV_T + 1], row[KV_T], have[KV_T], ws[KV_T / 64];
   __shared__ int64_t ws64[KV_T / 64];
@@ -182,7 +183,8 @@ __global__ __launch_bounds__(KV_T) void k_kv_extend(KvArgs kv, int n, const int3
 }
 
 // Pages of the listed sequences given back: all of them (window < 0), or those that no
-// later position of a sliding window with `sinks` first tokens sees.
+// later position of a sliding window with `sinks` first tokens sees.  A wave takes every 16th
+// sequence, one dependent load after the other: 3.7 us for 32 sequences, 34 for 1024.
 __global__ __launch_bounds__(KV_T) void k_kv_release(KvArgs kv, int n, const int32_t *seqs, int window, int sinks) {
   __shared__ int mark[KV_MAX_SEQS];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -648,8 +650,8 @@ __global__ __launch_bounds__(KV_T) void k_kv_write_check(KvArgs kv, KvWrite w) {
 // call that cannot be done writes nothing, whichever of them sets *status first; otherwise
 // k_kv_write_check has looked.
 // Bound by memory for prompts and by latency for single rows: 7900 rows of 32/4 heads of 128,
-// F16: 60 us, 5.1 TB/s, as a copy; 32 rows of 16/8 heads of 256, BF16: 5.8 us, 1 us of it the
-// look at the whole call.
+// F16: 55 us, 5.6 TB/s, and 5 us for k_kv_write_check; 32 rows of 16/8 heads of 256, BF16: 5.8 us,
+// 1 us of it the look at the whole call.
 template <int TYPE, int N, bool CHECK>
 __global__ __launch_bounds__(256) void k_kv_write(KvArgs kv, RopeArgs r, KvWrite w) {
   __shared__ WriteList l;
@@ -728,7 +730,8 @@ __global__ __launch_bounds__(256) void k_kv_write(KvArgs kv, RopeArgs r, KvWrite
   }
 }
 
-// Rows at given positions, as k_kv_write turns them; bound by memory.
+// Rows at given positions, as k_kv_write turns them; bound by memory: 7900 rows of 32 heads of
+// 128 take 39.5 us (259 MB, some of which stay in the last-level cache), 32 of 16 of 256 3.4 us.
 template <int N>
 __global__ __launch_bounds__(256) void k_rope(RopeArgs r, const float *x, float *out, int n_heads, int hs,
                                               const int32_t *positions) {

@@ -262,8 +262,10 @@ constexpr int prompt_ahead(int type) { return type == T_F32 ? 6 : 3; }
 // weights take (up to 168 a lane for heads up to 128, 256 up to 256, 512 beyond).  For heads up
 // to 128 a third wave on a SIMD has work where two wait for LDS and exponentials: 4096 tokens of
 // 16/4 heads take 222 us with 12 waves and 247 with 8 for 128 elements in F16, 157 and 188 for
-// 64, 258 and 267 for 128 in BF16 (which spills 4 registers); 16 waves
-// (128 registers) take as long for 64 elements and spill 35 for 128.
+// 64, 258 and 267 for 128 in BF16 (which spills 3 registers), and in F32 649 and 671 for 128
+// (which spills 37), 493 and 536 for 96, 346 and 375 for 64; 16 waves
+// (128 registers) take as long for 64 elements and spill 35 for 128.  Where F32 has few rows to a
+// sequence 8 waves are ahead for 128: 94 us against 117 for eight times 5 rows behind 4000.
 constexpr int prompt_waves(int hs) { return hs > 256 ? 4 : hs <= 128 ? 12 : 8; }
 constexpr int prompt_kt(int type, int hs) {
   const int es = type == T_F32 ? 4 : 2, kt = 32768 / (hs * es);

@@ -284,7 +284,8 @@ class Context:
         self.ordinal = ordinal
 
     def set_stream(self, stream_handle: Optional[int]) -> None:
-        """Launch *_dev work on an external hipStream_t (e.g. torch's current stream)."""
+        """Launch *_dev work on an external hipStream_t (e.g. torch's current stream).  None or 0,
+        the handle of torch's default stream: the context's own, which is not ordered with it."""
         check(lib().g4_ctx_set_stream(self.handle, stream_handle or None))
 
     def sync(self) -> None:
